@@ -54,6 +54,17 @@ class Stats(C.Structure):
         ("last_step_device_ms", C.c_double)]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in (
+        "k_pool", "v_pool", "key_bounds", "block_table", "seq_blocks", "free_blocks", "free_count")] + [(n, C.c_int32) for n in (
+        "n_blocks", "n_seqs", "max_blocks", "block_rows", "n_kv_heads", "head_dim")]
+
+
+class PagedRows(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("seq_row0", "row_slot", "row_pos", "slot_map", "status")] + [
+        ("n_rows", C.c_int32), ("_pad", C.c_int32)]
+
+
 # Every symbol include/b200_resident.h declares (the resident backend's boundary); the loader checks each one resolves.
 EXPORTS = (
     "b200_open", "b200_close", "b200_last_error", "b200_model_create", "b200_upload_tensor", "b200_set_rope_inv_freq",
@@ -64,6 +75,7 @@ EXPORTS = (
     "b200_op_quant_g32", "b200_op_q4k_dequant", "b200_op_q4k_matmul", "b200_op_q4k_quantize", "b200_op_f16_matmul",
     "b200_op_rmsnorm", "b200_op_route", "b200_op_draw", "b200_op_topk", "b200_op_philox", "b200_op_attention",
     "b200_op_prefill_attention", "b200_op_gate_up_swiglu", "b200_op_kq_matmul", "b200_attention_noalloc",
+    "b200_paged_plan", "b200_paged_append", "b200_paged_select", "b200_paged_attend",
 )
 
 # Every symbol include/b200_bench.h declares (measurement, synthetic workloads, test hooks).
@@ -71,5 +83,5 @@ BENCH_EXPORTS = (
     "b200_launch_count", "b200_synth_tensor", "b200_synth_kv", "b200_decode_loop_device", "b200_debug_read_hidden",
     "b200_profile", "b200_profile_read", "b200_bench_read", "b200_bench_kq_matmul", "b200_bench_q4k_matmul",
     "b200_bench_f16_matmul", "b200_bench_attention", "b200_bench_prefill_attention", "b200_debug_wait_fault", "b200_tp_fused_active", "b200_bench_tp_reduce", "b200_debug_q6k_matmul_umma", "b200_debug_kq_matmul_umma",
-    "b200_debug_tp_reduce_emulated",
+    "b200_debug_tp_reduce_emulated", "b200_debug_open_host",
 )

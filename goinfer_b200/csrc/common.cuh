@@ -133,6 +133,23 @@ struct PerDeviceOnce {
     }
 };
 
+// Makes `want` the calling thread's current device for the length of a call and puts the caller's own back afterwards.
+struct DeviceScope {
+    int prev = -1;
+    bool switched = false;
+    cudaError_t enter(int want) {
+        cudaError_t e = cudaGetDevice(&prev);
+        if (e != cudaSuccess) return e;
+        if (prev == want) return cudaSuccess;
+        e = cudaSetDevice(want);
+        switched = e == cudaSuccess;
+        return e;
+    }
+    ~DeviceScope() {
+        if (switched) cudaSetDevice(prev);
+    }
+};
+
 // ---- programmatic dependent launch -------------------------------------------------------------------------------
 // A kernel launched with launch_pdl may start while the kernel before it on the stream is still running: its blocks are
 // placed as soon as every block of the earlier kernel has called pdl_trigger() (or left), and they must call pdl_wait()

@@ -800,6 +800,15 @@ int b200_open(int device_ordinal, void* stream, b200_ctx** out) {
     return B200_OK;
 }
 
+int b200_debug_open_host(b200_ctx** out) {
+    if (!out) return B200_BAD_ARGUMENT;
+    auto* ctx = new (std::nothrow) b200_ctx();
+    if (!ctx) return B200_CUDA_ERROR;
+    ctx->device = -1;
+    *out = ctx;
+    return B200_OK;
+}
+
 void b200_close(b200_ctx* ctx) {
     if (!ctx) return;
     b200_tp_destroy(ctx);

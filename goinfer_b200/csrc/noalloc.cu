@@ -25,25 +25,6 @@ float* g_scratch_ptr[kMaxDevices] = {};
 std::mutex g_setup_mutex;
 }  // namespace
 
-namespace {
-// Makes `want` the calling thread's current device for the length of a call and puts the caller's own back afterwards.
-struct DeviceScope {
-    int prev = -1;
-    bool switched = false;
-    cudaError_t enter(int want) {
-        cudaError_t e = cudaGetDevice(&prev);
-        if (e != cudaSuccess) return e;
-        if (prev == want) return cudaSuccess;
-        e = cudaSetDevice(want);
-        switched = e == cudaSuccess;
-        return e;
-    }
-    ~DeviceScope() {
-        if (switched) cudaSetDevice(prev);
-    }
-};
-}  // namespace
-
 extern "C" int b200_attention_noalloc(b200_ctx* ctx, const float* q, int ldq, int rows, int n_heads, int n_kv_heads,
                                       int head_dim, float scale, float softcap, const int32_t* row_slot,
                                       const int32_t* row_pos, int max_keys, const void* k_pool, const void* v_pool,

@@ -1,0 +1,326 @@
+// paged.cu — a paged KV cache in the caller's own device memory: the block tables, free stack, packed rows and slot map
+// of a step from its request lengths (b200_paged_plan), and the store of a step's K/V rows with the bounds of their keys
+// (b200_paged_append).
+//
+// plan. Sequence i keeps len_i rows and takes new_i more, in blocks of br rows:
+//     want_i = ceil((len_i + new_i) / br),  grow_i = max(0, want_i - have_i),  shrink_i = max(0, have_i - want_i)
+// With G = sum grow and S = sum shrink, element e of the released blocks (sequence, then table position, ascending) is
+// pushed as number S-1-e, and element k of the new blocks is popped as number k: what the k-th new block pops is
+// stack[count + S - 1 - k], which for k < S is the k-th released block. Three scans (rows, grow, shrink) over the sequences
+// place everything; each released block, new block and row then finds its sequence by a search in the scan.
+// The kernel is latency: one launch of one cluster, whose CTAs each make the scans for themselves (a few ints a sequence)
+// and share the elements out. Cluster barriers stand between the reads of the old state, the pushes and the pops.
+#include "paged.cuh"
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanMaxSeqs = 16384;  // three scans of 4 bytes a sequence in shared memory
+
+struct PlanArgs {
+    int32_t* table;
+    int32_t* seq_blocks;
+    int32_t* stack;
+    int32_t* count;
+    const int32_t* kv_len;
+    const int32_t* n_new;
+    int32_t *row0, *row_slot, *row_pos, *slot_map, *status;
+    int n_seqs, n_blocks, max_blocks, block_rows, n_rows;
+};
+
+// the last index i with scan[i] <= e, for e < scan[n] (empty sequences are stepped over)
+__device__ __forceinline__ int find_owner(const int* scan, int n, int e) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (scan[mid] <= e) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+struct Sums {
+    long long rows;
+    int grow, shrink;
+};
+
+__device__ __forceinline__ Sums warp_inclusive(Sums v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long r = __shfl_up_sync(0xffffffffu, v.rows, o);
+        const int g = __shfl_up_sync(0xffffffffu, v.grow, o), s = __shfl_up_sync(0xffffffffu, v.shrink, o);
+        if (lane >= o) { v.rows += r; v.grow += g; v.shrink += s; }
+    }
+    return v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs a) {
+    extern __shared__ int plan_smem[];
+    int* row0 = plan_smem;                    // [n + 1] scan of new rows
+    int* grow0 = row0 + a.n_seqs + 1;         // [n + 1] scan of blocks taken
+    int* shrink0 = grow0 + a.n_seqs + 1;      // [n + 1] scan of blocks given back
+    __shared__ Sums warp_sum[32];
+    __shared__ int first_bad;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n_seqs, br = a.block_rows;
+    if (tid == 0) first_bad = n;
+    __syncthreads();
+
+    // every thread takes a run of sequences; two reads of the lengths, the second from the cache
+    const int per = (n + kPlanThreads - 1) / kPlanThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
+    auto look = [&](int i, int& want, int& have) {
+        const int len = a.kv_len[i], add = a.n_new[i];
+        have = a.seq_blocks[i];
+        const long long all = (long long)len + add;
+        const bool bad = len < 0 || add < 0 || all > (long long)a.max_blocks * br || have < 0 || have > a.max_blocks || len > (long long)have * br;
+        want = bad ? have : (int)((all + br - 1) / br);
+        return !bad;
+    };
+    Sums mine{0, 0, 0};
+    for (int i = i0; i < i1; i++) {
+        int want, have;
+        if (!look(i, want, have)) { atomicMin(&first_bad, i); continue; }
+        mine.rows += a.n_new[i];
+        mine.grow += max(0, want - have);
+        mine.shrink += max(0, have - want);
+    }
+    Sums scan = warp_inclusive(mine, lane);
+    if (lane == 31) warp_sum[warp] = scan;
+    __syncthreads();
+    if (warp == 0) {
+        const Sums t = warp_inclusive(warp_sum[lane], lane);
+        warp_sum[lane] = t;
+    }
+    __syncthreads();
+    const Sums total = warp_sum[31];
+    scan.rows -= mine.rows;
+    scan.grow -= mine.grow;
+    scan.shrink -= mine.shrink;
+    if (warp > 0) {
+        scan.rows += warp_sum[warp - 1].rows;
+        scan.grow += warp_sum[warp - 1].grow;
+        scan.shrink += warp_sum[warp - 1].shrink;
+    }
+    for (int i = i0; i < i1; i++) {
+        int want, have;
+        const bool good = look(i, want, have);
+        row0[i] = (int)scan.rows;  // used only when the rows fit n_rows
+        grow0[i] = scan.grow;
+        shrink0[i] = scan.shrink;
+        if (good) {
+            scan.rows += a.n_new[i];
+            scan.grow += max(0, want - have);
+            scan.shrink += max(0, have - want);
+        }
+    }
+    if (tid == 0) {
+        row0[n] = (int)total.rows;
+        grow0[n] = total.grow;
+        shrink0[n] = total.shrink;
+    }
+    const int free0 = *a.count, G = total.grow, S = total.shrink;
+    const int bad_seq = first_bad;
+    const bool bad = bad_seq < n || total.rows > a.n_rows || free0 < 0 || (long long)free0 + S > a.n_blocks;
+    const bool full = !bad && G > free0 + S;
+    const int rank = (int)cluster_rank(), ctas = (int)cluster_size();
+    const int gtid = rank * kPlanThreads + tid, step = ctas * kPlanThreads;
+    cluster_sync();  // the old state has been read by every CTA
+
+    if (rank == 0 && tid == 0) {
+        a.status[0] = bad ? B200_BAD_ARGUMENT : full ? B200_KV_POOL_FULL : B200_OK;
+        a.status[1] = bad || full ? 0 : (int)total.rows;
+        a.status[2] = bad || full ? free0 : free0 + S - G;
+        a.status[3] = bad ? bad_seq : full ? G - free0 - S : 0;
+        if (!bad && !full) *a.count = free0 + S - G;
+    }
+    if (bad || full) {  // nothing changes, and no row takes part in what follows
+        for (int r = gtid; r < a.n_rows; r += step) a.row_slot[r] = a.row_pos[r] = a.slot_map[r] = -1;
+        for (int i = gtid; i <= n; i += step) a.row0[i] = 0;
+        return;
+    }
+    auto want_of = [&](int i) { return (int)(((unsigned)a.kv_len[i] + (unsigned)a.n_new[i] + (unsigned)br - 1u) / (unsigned)br); };
+    for (int e = gtid; e < S; e += step) {
+        const int i = find_owner(shrink0, n, e);
+        int32_t* entry = a.table + (size_t)i * a.max_blocks + want_of(i) + (e - shrink0[i]);
+        a.stack[free0 + S - 1 - e] = *entry;
+        *entry = 0;
+    }
+    if (rank == 0)
+        for (int i = tid; i < n; i += kPlanThreads) a.seq_blocks[i] = want_of(i);
+    for (int i = gtid; i <= n; i += step) a.row0[i] = row0[i];
+    cluster_sync();  // the pushes are on the stack
+
+    for (int k = gtid; k < G; k += step) {
+        const int i = find_owner(grow0, n, k);
+        const int have = want_of(i) - (grow0[i + 1] - grow0[i]);
+        a.table[(size_t)i * a.max_blocks + have + (k - grow0[i])] = __ldcg(a.stack + free0 + S - 1 - k);
+    }
+    for (int r = gtid; r < a.n_rows; r += step) {
+        int slot = -1, pos = -1, at = -1;
+        if (r < (int)total.rows) {
+            slot = find_owner(row0, n, r);
+            pos = a.kv_len[slot] + r - row0[slot];
+            const int p = pos / br, grown = grow0[slot + 1] - grow0[slot], have = want_of(slot) - grown;
+            // a new block is read off the stack: its table entry may be another CTA's to write
+            const int block = p >= have && grown > 0 ? __ldcg(a.stack + free0 + S - 1 - (grow0[slot] + p - have))
+                                                      : a.table[(size_t)slot * a.max_blocks + p];
+            if (paged_block_ok(block, a.n_blocks)) at = block * br + pos % br;
+        }
+        a.row_slot[r] = slot;
+        a.row_pos[r] = pos;
+        a.slot_map[r] = at;
+    }
+}
+
+// ---- append ----------------------------------------------------------------------------------------------------------
+// Packed rows whose slots follow one another inside one block are a run; the first row of a run stores the whole run, so a
+// block's bounds are written once and see every key: lo_d = min, hi_d = max over the block's rows 0 .. last of the fp16
+// keys, the older ones read back from the pool. NaN keys make NaN bounds (min.NaN / max.NaN). A warp takes (run, kv head),
+// a lane HD/32 dims. Bytes bound it: 8 HD in and 4 HD out a row and head.
+__device__ __forceinline__ unsigned min_nan2(unsigned a, unsigned b) {
+    unsigned r;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned max_nan2(unsigned a, unsigned b) {
+    unsigned r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+template <int HD>
+struct LaneRow;  // a lane's share of a row: HD/32 floats in, as many halves out
+template <>
+struct LaneRow<128> {
+    using In = float4;
+    using Out = uint2;
+    static __device__ __forceinline__ Out pack(In x) {
+        const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+        return make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+    }
+    static __device__ __forceinline__ void fold(Out& lo, Out& hi, Out x) {
+        lo.x = min_nan2(lo.x, x.x); lo.y = min_nan2(lo.y, x.y);
+        hi.x = max_nan2(hi.x, x.x); hi.y = max_nan2(hi.y, x.y);
+    }
+};
+template <>
+struct LaneRow<64> {
+    using In = float2;
+    using Out = unsigned;
+    static __device__ __forceinline__ Out pack(In x) {
+        const __half2 a = __floats2half2_rn(x.x, x.y);
+        return *reinterpret_cast<const unsigned*>(&a);
+    }
+    static __device__ __forceinline__ void fold(Out& lo, Out& hi, Out x) { lo = min_nan2(lo, x); hi = max_nan2(hi, x); }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(256) paged_append_kernel(const b200_paged_cache c, const int32_t* __restrict__ slot_map, int n_rows,
+                                                           const float* __restrict__ k, size_t ldk, const float* __restrict__ v, size_t ldv) {
+    using L = LaneRow<HD>;
+    using In = typename L::In;
+    using Out = typename L::Out;
+    const int r = blockIdx.x, lane = threadIdx.x & 31, br = c.block_rows;
+    const int at = slot_map[r];
+    if (at < 0 || !paged_block_ok(at / br, c.n_blocks)) return;
+    const int block = at / br, first = at % br;
+    if (first > 0 && r > 0 && slot_map[r - 1] == at - 1) return;  // an earlier row of the run stores this one
+    int n = 1;
+    while (first + n < br && r + n < n_rows && slot_map[r + n] == at + n) n++;
+    for (int h = threadIdx.x >> 5; h < c.n_kv_heads; h += blockDim.x >> 5) {
+        const size_t tile = paged_tile(block, h, c.n_kv_heads, br, HD);
+        Out* kt = reinterpret_cast<Out*>(static_cast<__half*>(c.k_pool) + tile) + lane;
+        Out* vt = reinterpret_cast<Out*>(static_cast<__half*>(c.v_pool) + tile) + lane;
+        constexpr int RS = 32;  // Out elements between rows of a tile
+        Out lo, hi;
+        for (int j = 0; j < n; j++) {
+            const Out ko = L::pack(reinterpret_cast<const In*>(k + (size_t)(r + j) * ldk + (size_t)h * HD)[lane]);
+            const Out vo = L::pack(reinterpret_cast<const In*>(v + (size_t)(r + j) * ldv + (size_t)h * HD)[lane]);
+            kt[(first + j) * RS] = ko;
+            vt[(first + j) * RS] = vo;
+            if (j == 0) { lo = ko; hi = ko; }
+            else L::fold(lo, hi, ko);
+        }
+        if (!c.key_bounds) continue;
+        for (int j = 0; j < first; j++) L::fold(lo, hi, kt[j * RS]);
+        Out* b = reinterpret_cast<Out*>(static_cast<__half*>(c.key_bounds) + ((size_t)block * c.n_kv_heads + h) * 2 * HD) + lane;
+        b[0] = lo;
+        b[RS] = hi;
+    }
+}
+
+}  // namespace
+
+int paged_check(b200_ctx* ctx, const char* what, const b200_paged_cache* c, const b200_paged_rows* r, PagedNeeds need) {
+    if (!c || !r) B200_FAIL(ctx, B200_BAD_ARGUMENT, "%s: null cache or rows", what);
+    if (c->n_seqs < 1 || c->max_blocks < 1 || c->n_blocks < 2 || c->block_rows < 16 || c->block_rows > 256 || c->block_rows % 16 != 0)
+        B200_FAIL(ctx, B200_BAD_ARGUMENT,
+                  "%s: %d sequences of %d table entries over %d blocks of %d rows; a cache has at least one sequence and entry, two blocks "
+                  "(block 0 is the null block) and blocks of 16 to 256 rows, a multiple of 16", what, c->n_seqs, c->max_blocks, c->n_blocks, c->block_rows);
+    if ((long long)c->n_blocks * c->block_rows > 0x7fffffffLL || (long long)c->max_blocks * c->block_rows > 0x7fffffffLL)
+        B200_FAIL(ctx, B200_BAD_ARGUMENT, "%s: a pool and a table hold fewer than 2^31 rows each", what);
+    if (!c->block_table || paged_misaligned(c->block_table, 4)) B200_FAIL(ctx, B200_BAD_ARGUMENT, "%s: block_table is null or not 4-byte aligned", what);
+    if (r->n_rows < 0 || r->n_rows > 1 << 27) B200_FAIL(ctx, B200_BAD_ARGUMENT, "%s: %d rows; at most 2^27", what, r->n_rows);
+    if (r->n_rows > 0 && (need.stack || !need.map) && (!r->row_slot || !r->row_pos || paged_misaligned(r->row_slot, 4) || paged_misaligned(r->row_pos, 4)))
+        B200_FAIL(ctx, B200_BAD_ARGUMENT, "%s: row_slot or row_pos is null or not 4-byte aligned", what);
+    if (need.map && r->n_rows > 0 && (!r->slot_map || paged_misaligned(r->slot_map, 4)))
+        B200_FAIL(ctx, B200_BAD_ARGUMENT, "%s: slot_map is null or not 4-byte aligned", what);
+    if (need.stack) {
+        if (!c->seq_blocks || !c->free_blocks || !c->free_count || !r->seq_row0 || !r->status || paged_misaligned(c->seq_blocks, 4) ||
+            paged_misaligned(c->free_blocks, 4) || paged_misaligned(c->free_count, 4) || paged_misaligned(r->seq_row0, 4) || paged_misaligned(r->status, 4))
+            B200_FAIL(ctx, B200_BAD_ARGUMENT, "%s: seq_blocks, free_blocks, free_count, seq_row0 or status is null or not 4-byte aligned", what);
+    }
+    if (need.pools || need.bounds) {
+        if (c->n_kv_heads < 1 || !(c->head_dim == 64 || c->head_dim == 128))
+            B200_FAIL(ctx, B200_BAD_ARGUMENT, "%s: %d kv heads of %d; head_dim is 64 or 128", what, c->n_kv_heads, c->head_dim);
+        if (need.pools && (!c->k_pool || !c->v_pool || paged_misaligned(c->k_pool, 16) || paged_misaligned(c->v_pool, 16)))
+            B200_FAIL(ctx, B200_BAD_ARGUMENT, "%s: a pool is null or not 16-byte aligned", what);
+        if (need.bounds ? (!c->key_bounds || paged_misaligned(c->key_bounds, 16)) : paged_misaligned(c->key_bounds, 16))
+            B200_FAIL(ctx, B200_BAD_ARGUMENT, "%s: key_bounds is null or not 16-byte aligned", what);
+    }
+    return B200_OK;
+}
+
+extern "C" int b200_paged_plan(b200_ctx* ctx, const b200_paged_cache* c, const b200_paged_rows* r, const int32_t* kv_len, const int32_t* n_new) {
+    if (!ctx) return B200_BAD_ARGUMENT;
+    PagedNeeds need;
+    need.stack = need.map = true;
+    ST_TRY(paged_check(ctx, "b200_paged_plan", c, r, need));
+    if (!kv_len || !n_new || paged_misaligned(kv_len, 4) || paged_misaligned(n_new, 4))
+        B200_FAIL(ctx, B200_BAD_ARGUMENT, "b200_paged_plan: kv_len or n_new is null or not 4-byte aligned");
+    if (c->n_seqs > kPlanMaxSeqs || (long long)c->n_seqs * c->max_blocks > 0x7fffffffLL)
+        B200_FAIL(ctx, B200_BAD_ARGUMENT, "b200_paged_plan: %d sequences of %d table entries; at most %d sequences and 2^31 - 1 entries in all", c->n_seqs,
+                  c->max_blocks, kPlanMaxSeqs);
+    if (ctx->device < 0) B200_FAIL(ctx, B200_CUDA_ERROR, "b200_paged_plan: the context has no device");
+    DeviceScope dev;
+    CUDA_TRY(ctx, dev.enter(ctx->device));
+    const PlanArgs a{c->block_table, c->seq_blocks, c->free_blocks, c->free_count, kv_len, n_new, r->seq_row0, r->row_slot, r->row_pos, r->slot_map,
+                     r->status, c->n_seqs, c->n_blocks, c->max_blocks, c->block_rows, r->n_rows};
+    static SmemLimit limit;
+    const size_t smem = 3 * sizeof(int) * ((size_t)c->n_seqs + 1);
+    CUDA_TRY(ctx, limit.raise(paged_plan_kernel, ctx->device, 3 * sizeof(int) * (kPlanMaxSeqs + 1)));
+    const int ctas = 8;
+    launch_cluster(paged_plan_kernel, ctas, dim3(ctas), dim3(kPlanThreads), smem, ctx->stream, a);
+    LAUNCH_CHECK(ctx);
+    return B200_OK;
+}
+
+extern "C" int b200_paged_append(b200_ctx* ctx, const b200_paged_cache* c, const b200_paged_rows* r, const float* k, int ldk, const float* v, int ldv) {
+    if (!ctx) return B200_BAD_ARGUMENT;
+    PagedNeeds need;
+    need.pools = need.map = true;
+    ST_TRY(paged_check(ctx, "b200_paged_append", c, r, need));
+    if (r->n_rows == 0) return B200_OK;
+    const long long width = (long long)c->n_kv_heads * c->head_dim;
+    if (!k || !v || paged_misaligned(k, 16) || paged_misaligned(v, 16) || ldk < width || ldv < width || (ldk & 3) || (ldv & 3))
+        B200_FAIL(ctx, B200_BAD_ARGUMENT,
+                  "b200_paged_append: k and v must be 16-byte aligned with strides of at least %lld floats, a multiple of 4 (got %d and %d)", width, ldk, ldv);
+    if (ctx->device < 0) B200_FAIL(ctx, B200_CUDA_ERROR, "b200_paged_append: the context has no device");
+    DeviceScope dev;
+    CUDA_TRY(ctx, dev.enter(ctx->device));
+    const int warps = c->n_kv_heads < 8 ? c->n_kv_heads : 8;
+    if (c->head_dim == 128)
+        paged_append_kernel<128><<<r->n_rows, warps * 32, 0, ctx->stream>>>(*c, r->slot_map, r->n_rows, k, (size_t)ldk, v, (size_t)ldv);
+    else
+        paged_append_kernel<64><<<r->n_rows, warps * 32, 0, ctx->stream>>>(*c, r->slot_map, r->n_rows, k, (size_t)ldk, v, (size_t)ldv);
+    LAUNCH_CHECK(ctx);
+    return B200_OK;
+}

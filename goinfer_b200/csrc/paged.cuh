@@ -1,0 +1,94 @@
+// paged.cuh — what the operators over a caller-owned paged cache (paged.cu, paged_select.cu, paged_attend.cu) share:
+// address rules that hold on the host and on the device, cluster primitives, the checks of the host structs.
+#pragma once
+#include <atomic>
+
+#include "common.cuh"
+
+// A table entry names a block of the pools when it lies in 1 .. n_blocks-1 (block 0 is the null block). Every kernel asks
+// this before it forms an address, so a table that holds anything else reads and writes nothing.
+__host__ __device__ inline bool paged_block_ok(int block, int n_blocks) { return block > 0 && block < n_blocks; }
+
+// A packed row takes part when it names a sequence and a position; the rows behind the last sequence are marked -1.
+__host__ __device__ inline bool paged_row_ok(int slot, int pos, int n_seqs) { return slot >= 0 && slot < n_seqs && pos >= 0; }
+
+// Table positions that a row at `pos` sees (a position past the table sees the whole table).
+__host__ __device__ inline int paged_visible(int pos, int block_rows, int max_blocks) {
+    const int b = pos / block_rows;
+    return (b < max_blocks ? b : max_blocks - 1) + 1;
+}
+
+// Halves in front of row 0 of a block's tile of one kv head. 64-bit: a pool passes 2^31 elements at 4 GB.
+__host__ __device__ inline size_t paged_tile(int block, int kvh, int n_kv, int block_rows, int hd) {
+    return ((size_t)block * n_kv + kvh) * block_rows * hd;
+}
+
+// Checks of the structs that every entry point makes (paged.cu). need_*: which arrays the call touches.
+struct PagedNeeds {
+    bool pools = false, bounds = false, stack = false, map = false;
+};
+int paged_check(b200_ctx*, const char* what, const b200_paged_cache*, const b200_paged_rows*, PagedNeeds);
+
+inline bool paged_misaligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+// Raises a kernel's dynamic shared memory limit once per device. Two contexts of one device may come here at the same
+// time: the flag is set after the attribute, which may be set twice.
+struct SmemLimit {
+    std::atomic<bool> done[64] = {};
+    template <typename K>
+    cudaError_t raise(K* kernel, int device, size_t bytes) {
+        if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
+        if (done[device].load(std::memory_order_acquire)) return cudaSuccess;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == cudaSuccess) done[device].store(true, std::memory_order_release);
+        return e;
+    }
+};
+
+#ifdef __CUDACC__
+template <typename... KArgs, typename... Args>
+inline void launch_cluster(void (*kernel)(KArgs...), int cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);  // an error surfaces in LAUNCH_CHECK's cudaGetLastError
+}
+
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return r;
+}
+// All threads of the cluster; writes before it (global and shared) are visible behind it.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of a shared variable of this CTA in the CTA `rank` of the cluster.
+__device__ __forceinline__ unsigned cluster_addr(const void* p, unsigned rank) {
+    unsigned a = (unsigned)__cvta_generic_to_shared(p), r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float cluster_load_f32(unsigned addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_store_u64(unsigned addr, unsigned long long v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+#endif

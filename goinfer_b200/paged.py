@@ -1,0 +1,151 @@
+"""A paged KV cache in the caller's own device memory: the b200_paged_* entry points over device arrays.
+
+`PagedCache` is one layer's pools with the block tables and the free stack that every layer shares; `PagedRows` the packed
+rows of a step. Both are views: they check the arrays once and keep references to them, so a step costs one foreign call per
+operator. Arrays are anything with torch's tensor attributes (data_ptr, shape, stride, dtype, device, is_contiguous); the
+module itself imports no tensor library.
+
+    ops = Ops(0, stream=torch.cuda.current_stream().cuda_stream or 1)      # 1: the legacy default stream
+    cache = PagedCache(ops, table, seq_blocks, free_blocks, free_count, 16, k_pool, v_pool, key_bounds)
+    rows = PagedRows(row_slot, row_pos, slot_map, seq_row0, status)
+    cache.plan(kv_len, n_new, rows)
+    cache.append(rows, k, v)
+    cache.select(rows, q, sel)
+    cache.attend(rows, q, sel, out)
+
+Work is queued on the stream of `ops`, whatever the caller's current stream is; the two have to be ordered by the caller.
+Wrong arguments raise ResidentError with B200_BAD_ARGUMENT before anything is queued. What the lengths ask of the pool is
+known on the device only: `rows.status` says whether a plan went through (include/b200_resident.h).
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import abi
+from .resident import ResidentError
+
+
+def _refuse(text: str):
+    raise ResidentError(abi.BAD_ARGUMENT, text)
+
+
+def _array(name: str, a, dtype: str, shape, device: int):
+    """Address of a contiguous device array of this type and shape (None entries of shape: any extent)."""
+    if str(a.dtype) != dtype:
+        _refuse(f"{name} has type {a.dtype}, not {dtype}")
+    if len(a.shape) != len(shape) or any(w is not None and n != w for n, w in zip(a.shape, shape)):
+        _refuse(f"{name} has shape {tuple(a.shape)}, not {tuple('any' if w is None else w for w in shape)}")
+    if a.device.type != "cuda" or a.device.index != device:
+        _refuse(f"{name} is on {a.device}, the context on cuda:{device}")
+    if not a.is_contiguous():
+        _refuse(f"{name} is not contiguous")
+    return a.data_ptr()
+
+
+class PagedRows:
+    """The packed rows of a step: row_slot, row_pos [n_rows] int32, and what plan and append need besides."""
+
+    def __init__(self, row_slot, row_pos, slot_map=None, seq_row0=None, status=None):
+        device = row_slot.device.index if row_slot.device.type == "cuda" else -1
+        n = row_slot.shape[0]
+        self.n_rows, self.device = n, device
+        self.n_seqs = None if seq_row0 is None else seq_row0.shape[0] - 1
+        self._keep = (row_slot, row_pos, slot_map, seq_row0, status)
+        self.row_slot, self.row_pos, self.slot_map, self.seq_row0, self.status = self._keep
+        i32 = "torch.int32"
+        self.c = abi.PagedRows(None if seq_row0 is None else _array("seq_row0", seq_row0, i32, (None,), device),
+                               _array("row_slot", row_slot, i32, (n,), device), _array("row_pos", row_pos, i32, (n,), device),
+                               None if slot_map is None else _array("slot_map", slot_map, i32, (n,), device),
+                               None if status is None else _array("status", status, i32, (4,), device), n, 0)
+        self.ref = C.byref(self.c)
+
+
+class PagedCache:
+    """block_table [n_seqs][max_blocks], seq_blocks [n_seqs], free_blocks [n_blocks], free_count [1], all int32; k_pool, v_pool
+    fp16 [n_blocks][n_kv_heads][block_rows][head_dim]; key_bounds fp16 [n_blocks][n_kv_heads][2][head_dim]. A cache without
+    pools plans, one without key_bounds selects nothing and keeps no bounds as it appends."""
+
+    def __init__(self, ops, block_table, seq_blocks, free_blocks, free_count, block_rows: int, k_pool=None, v_pool=None, key_bounds=None):
+        self.ops, self.device = ops, ops.drv.device
+        dev, i32, f16 = self.device, "torch.int32", "torch.float16"
+        self._keep = (block_table, seq_blocks, free_blocks, free_count, k_pool, v_pool, key_bounds)
+        table = _array("block_table", block_table, i32, (None, None), dev)
+        self.n_seqs, max_blocks = block_table.shape
+        n_blocks = free_blocks.shape[0]
+        kv = hd = 0
+        if k_pool is not None or v_pool is not None:
+            if k_pool is None or v_pool is None:
+                _refuse("k_pool and v_pool come together")
+            if len(k_pool.shape) != 4:
+                _refuse(f"k_pool has shape {tuple(k_pool.shape)}, not [n_blocks][n_kv_heads][block_rows][head_dim]")
+            kv, hd = k_pool.shape[1], k_pool.shape[3]
+        elif key_bounds is not None:
+            if len(key_bounds.shape) != 4:
+                _refuse(f"key_bounds has shape {tuple(key_bounds.shape)}, not [n_blocks][n_kv_heads][2][head_dim]")
+            kv, hd = key_bounds.shape[1], key_bounds.shape[3]
+        pool = lambda name, a: None if a is None else _array(name, a, f16, (n_blocks, kv, block_rows, hd), dev)  # noqa: E731
+        self.block_rows, self.n_kv_heads, self.head_dim = block_rows, kv, hd
+        self.c = abi.PagedCache(pool("k_pool", k_pool), pool("v_pool", v_pool),
+                                None if key_bounds is None else _array("key_bounds", key_bounds, f16, (n_blocks, kv, 2, hd), dev), table,
+                                _array("seq_blocks", seq_blocks, i32, (self.n_seqs,), dev), _array("free_blocks", free_blocks, i32, (n_blocks,), dev),
+                                _array("free_count", free_count, i32, (1,), dev), n_blocks, self.n_seqs, max_blocks, block_rows, kv, hd)
+        self.ref = C.byref(self.c)
+        lib = ops.lib
+        vp, i, f = C.c_void_p, C.c_int, C.c_float
+        for fn, types in ((lib.b200_paged_plan, (vp, vp, vp, vp, vp)), (lib.b200_paged_append, (vp, vp, vp, vp, i, vp, i)),
+                          (lib.b200_paged_select, (vp, vp, vp, vp, i, i, i, i, i, vp)),
+                          (lib.b200_paged_attend, (vp, vp, vp, vp, i, i, f, f, vp, i, vp, i))):
+            fn.argtypes = types
+        self._plan, self._append, self._select, self._attend = lib.b200_paged_plan, lib.b200_paged_append, lib.b200_paged_select, lib.b200_paged_attend
+
+    def _check(self, st: int):
+        if st != abi.OK:
+            raise ResidentError(st, self.ops.drv.last_error())
+
+    def _rows2d(self, name: str, a, rows: PagedRows) -> int:
+        """Row stride of a f32 [n_rows][...] device array whose rows are contiguous."""
+        shape, stride = a.shape, a.stride()
+        inner = 1
+        for n, st in zip(shape[:0:-1], stride[:0:-1]):
+            if n != 1 and st != inner:
+                _refuse(f"the rows of {name} are not contiguous (shape {tuple(shape)}, strides {stride})")
+            inner *= n
+        if shape[0] != rows.n_rows or str(a.dtype) != "torch.float32" or a.device.type != "cuda" or a.device.index != self.device:
+            _refuse(f"{name} is {a.dtype} {tuple(shape)} on {a.device}, not f32 with {rows.n_rows} rows on cuda:{self.device}")
+        return stride[0] if shape[0] > 1 else inner
+
+    def _heads(self, q) -> int:
+        width = 1
+        for n in q.shape[1:]:
+            width *= n
+        if self.head_dim == 0 or width % self.head_dim:
+            _refuse(f"q has {width} values a row, not whole heads of {self.head_dim}")
+        return width // self.head_dim
+
+    def _lists(self, sel, rows: PagedRows):
+        p = _array("sel", sel, "torch.int32", (rows.n_rows, self.n_kv_heads, None), self.device)
+        return p, sel.shape[2]
+
+    def plan(self, kv_len, n_new, rows: PagedRows):
+        if rows.n_seqs != self.n_seqs or rows.device != self.device:
+            _refuse(f"rows are for {rows.n_seqs} sequences on cuda:{rows.device}, the cache has {self.n_seqs} on cuda:{self.device}")
+        n = (self.n_seqs,)
+        self._check(self._plan(self.ops.ctx, self.ref, rows.ref, _array("kv_len", kv_len, "torch.int32", n, self.device),
+                               _array("n_new", n_new, "torch.int32", n, self.device)))
+
+    def append(self, rows: PagedRows, k, v):
+        ldk, ldv = self._rows2d("k", k, rows), self._rows2d("v", v, rows)
+        if k.shape[1:] != v.shape[1:] or k[0:1].numel() != min(1, rows.n_rows) * self.n_kv_heads * self.head_dim:
+            _refuse(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have {self.n_kv_heads} heads of {self.head_dim} a row")
+        self._check(self._append(self.ops.ctx, self.ref, rows.ref, k.data_ptr(), ldk, v.data_ptr(), ldv))
+
+    def select(self, rows: PagedRows, q, sel, n_first: int = 1, n_recent: int = 1):
+        p, n = self._lists(sel, rows)
+        self._check(self._select(self.ops.ctx, self.ref, rows.ref, q.data_ptr(), self._rows2d("q", q, rows), self._heads(q), n_first, n_recent, n, p))
+
+    def attend(self, rows: PagedRows, q, sel, out, scale: float = 0.0, softcap: float = 0.0):
+        p, n = self._lists(sel, rows)
+        heads, ldo = self._heads(q), self._rows2d("out", out, rows)
+        if self._heads(out) != heads:
+            _refuse(f"out has shape {tuple(out.shape)}, q {tuple(q.shape)}")
+        self._check(self._attend(self.ops.ctx, self.ref, rows.ref, q.data_ptr(), self._rows2d("q", q, rows), heads, scale, softcap, p, n, out.data_ptr(), ldo))

@@ -125,6 +125,7 @@ class _B200Driver:
 
     def __init__(self, device: int = 0, stream: Optional[int] = None):
         self.lib = load_library()
+        self.device = device
         self.ctx = C.c_void_p()
         st = self.lib.b200_open(device, C.c_void_p(stream or 0), C.byref(self.ctx))
         if st != abi.OK:

@@ -95,6 +95,10 @@ int b200_bench_tp_reduce(b200_model* m, int T, int mode, int warmup, int iters, 
 int b200_debug_tp_reduce_emulated(b200_ctx* ctx, int t, int T, int H, const float* parts, const float* h, const float* w,
                                   float eps, int mode, int n_kparts, int8_t* codes_out, float* scales_out, float* h_out);
 
+/* Test hook: a context without a device, for the argument checks of the b200_paged_* calls where there is no GPU. A call
+ * that passes them returns B200_CUDA_ERROR; other entry points must not be given this context. b200_close frees it. */
+int b200_debug_open_host(b200_ctx** out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -347,6 +347,86 @@ int b200_attention_noalloc(b200_ctx* ctx, const float* q, int ldq, int rows, int
                            const void* k_pool, const void* v_pool, const int32_t* block_table, int max_blocks,
                            int block_rows, float* out);
 
+/* ---- a paged cache in the caller's own device memory ------------------------------------------------------------------
+ * b200_attention_noalloc reads pools, tables and row arrays that the caller owns. These four calls make and use them on the
+ * device: plan (block tables, free stack, packed rows and slot map from request lengths), append (the step's K/V rows and
+ * the bounds of their keys into the pools), select (the blocks of a long context worth reading for a query) and attend
+ * (attention over the selected blocks). No counterpart in the reference, whose pool lives inside its backend and whose
+ * attention reads every key (backend/cuda/kvpool.go:16-76, decoder/forwardn.go:295-501).
+ *
+ * All pointers in the structs and all arrays are DEVICE pointers of the context's device; the structs themselves are read
+ * during the call. Work is queued on the context's stream: what another stream wrote must be ordered before it, and the
+ * caller synchronizes before reading results on the host. Nothing is allocated, no scratch is kept and no host
+ * synchronization happens, so the calls may be captured into CUDA graphs, and calls on several contexts, streams or
+ * devices share nothing but the arrays they are given. The caller's current device is the same after a call as before.
+ * One call at a time per context. What the device arrays hold cannot be checked by the host: a table entry outside
+ * 1 .. n_blocks-1 counts as unmapped (its keys are not there), a packed row whose slot or position is negative, or whose
+ * slot is n_seqs or more, takes no part and its outputs stay as they were. B200_BAD_ARGUMENT names what does not fit in
+ * b200_last_error; nothing is queued then. */
+typedef struct {
+    void* k_pool;          /* fp16 [n_blocks][n_kv_heads][block_rows][head_dim], 16-byte aligned (append, attend)        */
+    void* v_pool;
+    void* key_bounds;      /* fp16 [n_blocks][n_kv_heads][2][head_dim], 16-byte aligned: per dim the least and the largest
+                              value of the block's keys (select); NULL: append keeps none                                */
+    int32_t* block_table;  /* [n_seqs][max_blocks]; 0 = unmapped                                                         */
+    int32_t* seq_blocks;   /* [n_seqs] table entries in use (plan)                                                       */
+    int32_t* free_blocks;  /* [n_blocks] stack of the free blocks, the top last (plan)                                   */
+    int32_t* free_count;   /* [1] how many it holds                                                                      */
+    int32_t n_blocks;      /* blocks in a pool, the null block 0 included; n_blocks * block_rows < 2^31                   */
+    int32_t n_seqs, max_blocks;
+    int32_t block_rows;    /* 16 .. 256, a multiple of 16                                                                */
+    int32_t n_kv_heads, head_dim; /* head_dim 64 or 128                                                                  */
+} b200_paged_cache;
+
+/* A step's packed rows. Written by plan; append reads slot_map, select and attend row_slot and row_pos. */
+typedef struct {
+    int32_t* seq_row0;     /* [n_seqs + 1] first packed row of each sequence                                             */
+    int32_t* row_slot;     /* [n_rows] the row's sequence, -1 behind the last one                                        */
+    int32_t* row_pos;      /* [n_rows] its position                                                                      */
+    int32_t* slot_map;     /* [n_rows] the pool row that holds it: block * block_rows + row in block                      */
+    int32_t* status;       /* [4], see b200_paged_plan                                                                   */
+    int32_t n_rows;        /* rows the arrays have room for (a captured step keeps it fixed); at most 2^27                */
+    int32_t _pad;
+} b200_paged_rows;
+
+/* Sequence i keeps its first kv_len[i] rows and takes n_new[i] more. Table entries past what they need go back to the free
+ * stack (pushed from the last sequence's last block down), entries they lack are popped from it (for the first sequence's
+ * first block up), released blocks first: growing and giving back the same blocks restores the stack. kv_len = n_new = 0
+ * retires a sequence; a kv_len below what is stored rewinds it. Then the packed rows are written: sequence after sequence,
+ * n_new[i] rows at positions kv_len[i] ...; the rows behind the last are -1 in all three arrays.
+ * All or nothing: status[0] is 0, B200_KV_POOL_FULL (the stack lacks blocks) or B200_BAD_ARGUMENT (a negative length, a
+ * sequence longer than its table, a kv_len beyond its blocks, more than n_rows rows, a free_count that cannot be); in the
+ * last two cases the tables, seq_blocks and the stack stay as they were, every row is -1 and seq_row0 is 0, so that the
+ * rest of a captured step does nothing. status[1]: packed rows; [2]: free blocks afterwards; [3]: 0, or the blocks that
+ * are missing, or the first sequence that does not fit (n_seqs when it is none of them).
+ * A block belongs to one table row. At most 16384 sequences. */
+int b200_paged_plan(b200_ctx* ctx, const b200_paged_cache* cache, const b200_paged_rows* rows, const int32_t* kv_len, const int32_t* n_new);
+
+/* Stores row r of k and v ([n_rows][ldk or ldv] f32, n_kv_heads * head_dim used, 16-byte aligned, strides a multiple of 4),
+ * rounded to fp16, at slot_map[r]; rows whose slot_map is negative or past the pools are left out. With key_bounds, the
+ * bounds of every block written to are then those of its rows 0 .. the last one written (rows behind it, left over from a
+ * rewound sequence, do not count; a NaN makes its bound NaN). slot_map as plan writes it: distinct, a block's rows next to
+ * one another in ascending order. */
+int b200_paged_append(b200_ctx* ctx, const b200_paged_cache* cache, const b200_paged_rows* rows, const float* k, int ldk, const float* v, int ldv);
+
+/* For every row and kv head, n_select table positions out of the blocks 0 .. row_pos / block_rows that the row sees, to
+ * sel [n_rows][n_kv_heads][n_select], ascending, -1 behind the last: all of them when they are no more than n_select, else
+ * the first n_first, the last n_recent (at least 1: the block being filled is not scored) and the best of those between by
+ *     score = max over the group's query heads of sum_d q_d * (q_d > 0 ? largest_d : least_d),
+ * the bound of q.k over the block's keys, compared in f64; ties go to the lower block. A NaN or infinite score counts as
+ * the largest finite value, an unmapped block as the lowest. q [n_rows][ldq] f32, 16-byte aligned, ldq a multiple of 4; a
+ * group has 1 to 8 query heads; n_select at most 2048, max_blocks at most 24576. */
+int b200_paged_select(b200_ctx* ctx, const b200_paged_cache* cache, const b200_paged_rows* rows, const float* q, int ldq, int n_heads,
+                      int n_first, int n_recent, int n_select, int32_t* sel);
+
+/* Attention of every row over the keys 0 .. row_pos of the blocks that its list names, per kv head: sel as select writes it,
+ * or any list of table positions (entries that are negative, or behind the row's position, are left out; one that is named
+ * twice counts twice). Scores are scale * q.k (scale 0: 1/sqrt(head_dim)), softcap > 0 caps them (decoder/attention.go:287-295);
+ * a row that sees no key gets zeros. q [n_rows][ldq] and out [n_rows][ldo] f32, 16-byte aligned, strides a multiple of 4,
+ * out apart from the inputs. fp32 accuracy over the fp16 cache. */
+int b200_paged_attend(b200_ctx* ctx, const b200_paged_cache* cache, const b200_paged_rows* rows, const float* q, int ldq, int n_heads,
+                      float scale, float softcap, const int32_t* sel, int n_select, float* out, int ldo);
+
 #ifdef __cplusplus
 }
 #endif

@@ -101,6 +101,18 @@ type statsC struct {
 	LastStepDeviceMs                                                     float64
 }
 
+// pagedCacheC mirrors b200_paged_cache (device pointers of the caller's own paged cache): 7 pointers then 6 int32, 80 bytes.
+type pagedCacheC struct {
+	KPool, VPool, KeyBounds, BlockTable, SeqBlocks, FreeBlocks, FreeCount unsafe.Pointer
+	NBlocks, NSeqs, MaxBlocks, BlockRows, NKVHeads, HeadDim               int32
+}
+
+// pagedRowsC mirrors b200_paged_rows: 5 pointers then 2 int32, 48 bytes.
+type pagedRowsC struct {
+	SeqRow0, RowSlot, RowPos, SlotMap, Status unsafe.Pointer
+	NRows, Pad                                int32
+}
+
 // One variable per symbol of include/b200_resident.h, in the header's order. Pointers into Go slices are passed as
 // unsafe.Pointer of the first element; the library reads them during the call only.
 var (
@@ -153,6 +165,12 @@ var (
 	b200OpKQMatmul      func(ctx unsafe.Pointer, kind int32, w *byte, x *float32, M, K, N int32, dst *float32) int32
 	b200AttentionNoAlloc func(ctx unsafe.Pointer, q *float32, ldq, rows, nHeads, nKVHeads, headDim int32, scale, softcap float32,
 		rowSlot, rowPos *int32, maxKeys int32, kPool, vPool unsafe.Pointer, table *int32, maxBlocks, blockRows int32, out *float32) int32
+	// a paged cache in the caller's own device memory (all arrays are device pointers)
+	b200PagedPlan   func(ctx unsafe.Pointer, cache *pagedCacheC, rows *pagedRowsC, kvLen, nNew unsafe.Pointer) int32
+	b200PagedAppend func(ctx unsafe.Pointer, cache *pagedCacheC, rows *pagedRowsC, k unsafe.Pointer, ldk int32, v unsafe.Pointer, ldv int32) int32
+	b200PagedSelect func(ctx unsafe.Pointer, cache *pagedCacheC, rows *pagedRowsC, q unsafe.Pointer, ldq, nHeads, nFirst, nRecent, nSelect int32, sel unsafe.Pointer) int32
+	b200PagedAttend func(ctx unsafe.Pointer, cache *pagedCacheC, rows *pagedRowsC, q unsafe.Pointer, ldq, nHeads int32, scale, softcap float32,
+		sel unsafe.Pointer, nSelect int32, out unsafe.Pointer, ldo int32) int32
 )
 
 var (
@@ -165,7 +183,8 @@ var (
 func load() error {
 	loadOnce.Do(func() {
 		if unsafe.Sizeof(modelCfg{}) != 116 || unsafe.Sizeof(drawC{}) != 24 || unsafe.Offsetof(drawC{}.U) != 16 ||
-			unsafe.Sizeof(capsC{}) != 56 || unsafe.Sizeof(statsC{}) != 56 {
+			unsafe.Sizeof(capsC{}) != 56 || unsafe.Sizeof(statsC{}) != 56 ||
+			unsafe.Sizeof(pagedCacheC{}) != 80 || unsafe.Sizeof(pagedRowsC{}) != 48 {
 			loadErr = errors.New("b200: a struct mirror no longer matches include/b200_resident.h")
 			return
 		}
@@ -195,6 +214,8 @@ func load() error {
 			{&b200OpAttention, "b200_op_attention"}, {&b200OpPrefillAttn, "b200_op_prefill_attention"},
 			{&b200OpGateUpSwiglu, "b200_op_gate_up_swiglu"}, {&b200OpKQMatmul, "b200_op_kq_matmul"},
 			{&b200AttentionNoAlloc, "b200_attention_noalloc"},
+			{&b200PagedPlan, "b200_paged_plan"}, {&b200PagedAppend, "b200_paged_append"},
+			{&b200PagedSelect, "b200_paged_select"}, {&b200PagedAttend, "b200_paged_attend"},
 		} {
 			purego.RegisterLibFunc(s.fptr, lib, s.name)
 		}
