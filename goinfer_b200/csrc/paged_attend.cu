@@ -11,7 +11,8 @@
 // Products run on mma.sync m16n8k16 over the fp16 cache with fp32 accumulation; f32 queries and weights are split into
 // fp16 hi + lo parts (x = hi + lo to 2^-22), so the result keeps fp32 accuracy. S[head][key] = Q K^T takes the group's
 // heads as rows; the context is accumulated transposed, O^T[dim][head] = V^T P^T, where a lane's scores are already the
-// second operand. Rows of the last tile behind the position are filled with zeros by the copy: what the pool holds there
+// second operand. A tile's context starts from zero and is added to the running one by a rounded fma: the matrix unit cuts off
+// what it adds to, and over the tiles of a long list that went one way (2048 keys: 1.5e-6 of the result, 3e-7 so). Rows of the last tile behind the position are filled with zeros by the copy: what the pool holds there
 // (a NaN, say) meets a weight of 0 and must not be multiplied.
 #include "paged.cuh"
 
@@ -199,11 +200,15 @@ __global__ void __launch_bounds__(kAttThreads) paged_attend_kernel(const b200_pa
         const float a0 = __shfl_sync(0xffffffffu, alpha, (2 * tig) * 4), a1 = __shfl_sync(0xffffffffu, alpha, (2 * tig + 1) * 4);
 #pragma unroll
         for (int mt = 0; mt < KS; mt++) {
-            o[mt][0] *= a0; o[mt][1] *= a1; o[mt][2] *= a0; o[mt][3] *= a1;
             unsigned v[4];
             ldm4_t(vb + (unsigned)(lrow * ROWB + (((2 * mt + lsel) ^ (lrow & 7)) << 4)), v);
-            mma16816(o[mt], v[0], v[1], v[2], v[3], ph0, ph1);
-            mma16816(o[mt], v[0], v[1], v[2], v[3], pl0, pl1);
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma16816(d, v[0], v[1], v[2], v[3], pl0, pl1);
+            mma16816(d, v[0], v[1], v[2], v[3], ph0, ph1);
+            o[mt][0] = fmaf(o[mt][0], a0, d[0]);
+            o[mt][1] = fmaf(o[mt][1], a1, d[1]);
+            o[mt][2] = fmaf(o[mt][2], a0, d[2]);
+            o[mt][3] = fmaf(o[mt][3], a1, d[3]);
         }
         __syncwarp();
     }
