@@ -2,7 +2,7 @@
 
 `PagedCache` is one layer's pools with the block tables and the free stack that every layer shares; `PagedRows` the packed
 rows of a step. Both are views: they check the arrays once and keep references to them, so a step costs one foreign call per
-operator. Arrays are anything with torch's tensor attributes (data_ptr, shape, stride, dtype, device, is_contiguous); the
+operator. Arrays are anything with torch's tensor attributes (data_ptr, shape, stride, dtype, get_device, is_contiguous); the
 module itself imports no tensor library.
 
     ops = Ops(0, stream=torch.cuda.current_stream().cuda_stream or 1)      # 1: the legacy default stream
@@ -29,13 +29,23 @@ def _refuse(text: str):
     raise ResidentError(abi.BAD_ARGUMENT, text)
 
 
+_NAMES: dict = {}  # dtype -> its text (formatting one costs more than a whole check)
+
+
+def _is(dtype, name: str) -> bool:
+    text = _NAMES.get(dtype)
+    if text is None:
+        text = _NAMES[dtype] = str(dtype)
+    return text == name
+
+
 def _array(name: str, a, dtype: str, shape, device: int):
     """Address of a contiguous device array of this type and shape (None entries of shape: any extent)."""
-    if str(a.dtype) != dtype:
+    if not _is(a.dtype, dtype):
         _refuse(f"{name} has type {a.dtype}, not {dtype}")
-    if len(a.shape) != len(shape) or any(w is not None and n != w for n, w in zip(a.shape, shape)):
+    if a.shape != shape and (len(a.shape) != len(shape) or any(w is not None and n != w for n, w in zip(a.shape, shape))):
         _refuse(f"{name} has shape {tuple(a.shape)}, not {tuple('any' if w is None else w for w in shape)}")
-    if a.device.type != "cuda" or a.device.index != device:
+    if a.get_device() != device:
         _refuse(f"{name} is on {a.device}, the context on cuda:{device}")
     if not a.is_contiguous():
         _refuse(f"{name} is not contiguous")
@@ -46,7 +56,9 @@ class PagedRows:
     """The packed rows of a step: row_slot, row_pos [n_rows] int32, and what plan and append need besides."""
 
     def __init__(self, row_slot, row_pos, slot_map=None, seq_row0=None, status=None):
-        device = row_slot.device.index if row_slot.device.type == "cuda" else -1
+        device = row_slot.get_device()
+        if device < 0:
+            _refuse(f"row_slot is on {row_slot.device}")
         n = row_slot.shape[0]
         self.n_rows, self.device = n, device
         self.n_seqs = None if seq_row0 is None else seq_row0.shape[0] - 1
@@ -98,54 +110,63 @@ class PagedCache:
             fn.argtypes = types
         self._plan, self._append, self._select, self._attend = lib.b200_paged_plan, lib.b200_paged_append, lib.b200_paged_select, lib.b200_paged_attend
 
-    def _check(self, st: int):
-        if st != abi.OK:
-            raise ResidentError(st, self.ops.drv.last_error())
+    def _raise(self, st: int):
+        raise ResidentError(st, self.ops.drv.last_error())
 
-    def _rows2d(self, name: str, a, rows: PagedRows) -> int:
-        """Row stride of a f32 [n_rows][...] device array whose rows are contiguous."""
-        shape, stride = a.shape, a.stride()
-        inner = 1
-        for n, st in zip(shape[:0:-1], stride[:0:-1]):
-            if n != 1 and st != inner:
-                _refuse(f"the rows of {name} are not contiguous (shape {tuple(shape)}, strides {stride})")
-            inner *= n
-        if shape[0] != rows.n_rows or str(a.dtype) != "torch.float32" or a.device.type != "cuda" or a.device.index != self.device:
-            _refuse(f"{name} is {a.dtype} {tuple(shape)} on {a.device}, not f32 with {rows.n_rows} rows on cuda:{self.device}")
-        return stride[0] if shape[0] > 1 else inner
-
-    def _heads(self, q) -> int:
-        width = 1
-        for n in q.shape[1:]:
-            width *= n
-        if self.head_dim == 0 or width % self.head_dim:
-            _refuse(f"q has {width} values a row, not whole heads of {self.head_dim}")
-        return width // self.head_dim
+    def _packed(self, name: str, a, rows: PagedRows):
+        """Address, row stride and row width of a f32 [n_rows][...] device array whose rows are contiguous."""
+        shape, stride, n_rows = a.shape, a.stride(), rows.n_rows
+        if len(shape) == 2 and stride[1] == 1:
+            width = shape[1]
+        else:
+            width = 1
+            for n, st in zip(shape[:0:-1], stride[:0:-1]):
+                if n != 1 and st != width:
+                    _refuse(f"the rows of {name} are not contiguous (shape {tuple(shape)}, strides {stride})")
+                width *= n
+        if shape[0] != n_rows or not _is(a.dtype, "torch.float32") or a.get_device() != self.device or rows.device != self.device:
+            _refuse(f"{name} is {a.dtype} {tuple(shape)} on {a.device}, not f32 with {n_rows} rows on cuda:{self.device}, or the rows are not there")
+        return a.data_ptr(), stride[0] if n_rows > 1 else width, width
 
     def _lists(self, sel, rows: PagedRows):
-        p = _array("sel", sel, "torch.int32", (rows.n_rows, self.n_kv_heads, None), self.device)
-        return p, sel.shape[2]
+        shape = sel.shape
+        return _array("sel", sel, "torch.int32", (rows.n_rows, self.n_kv_heads, shape[-1]), self.device), shape[-1]
+
+    def _heads(self, name: str, width: int) -> int:
+        if self.head_dim == 0 or width % self.head_dim:
+            _refuse(f"{name} has {width} values a row, not whole heads of {self.head_dim}")
+        return width // self.head_dim
 
     def plan(self, kv_len, n_new, rows: PagedRows):
         if rows.n_seqs != self.n_seqs or rows.device != self.device:
             _refuse(f"rows are for {rows.n_seqs} sequences on cuda:{rows.device}, the cache has {self.n_seqs} on cuda:{self.device}")
-        n = (self.n_seqs,)
-        self._check(self._plan(self.ops.ctx, self.ref, rows.ref, _array("kv_len", kv_len, "torch.int32", n, self.device),
-                               _array("n_new", n_new, "torch.int32", n, self.device)))
+        st = self._plan(self.ops.ctx, self.ref, rows.ref, _array("kv_len", kv_len, "torch.int32", (self.n_seqs,), self.device),
+                        _array("n_new", n_new, "torch.int32", (self.n_seqs,), self.device))
+        if st:
+            self._raise(st)
 
     def append(self, rows: PagedRows, k, v):
-        ldk, ldv = self._rows2d("k", k, rows), self._rows2d("v", v, rows)
-        if k.shape[1:] != v.shape[1:] or k[0:1].numel() != min(1, rows.n_rows) * self.n_kv_heads * self.head_dim:
+        pk, ldk, wk = self._packed("k", k, rows)
+        pv, ldv, wv = self._packed("v", v, rows)
+        if wk != self.n_kv_heads * self.head_dim or wv != wk:
             _refuse(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have {self.n_kv_heads} heads of {self.head_dim} a row")
-        self._check(self._append(self.ops.ctx, self.ref, rows.ref, k.data_ptr(), ldk, v.data_ptr(), ldv))
+        st = self._append(self.ops.ctx, self.ref, rows.ref, pk, ldk, pv, ldv)
+        if st:
+            self._raise(st)
 
     def select(self, rows: PagedRows, q, sel, n_first: int = 1, n_recent: int = 1):
         p, n = self._lists(sel, rows)
-        self._check(self._select(self.ops.ctx, self.ref, rows.ref, q.data_ptr(), self._rows2d("q", q, rows), self._heads(q), n_first, n_recent, n, p))
+        pq, ldq, width = self._packed("q", q, rows)
+        st = self._select(self.ops.ctx, self.ref, rows.ref, pq, ldq, self._heads("q", width), n_first, n_recent, n, p)
+        if st:
+            self._raise(st)
 
     def attend(self, rows: PagedRows, q, sel, out, scale: float = 0.0, softcap: float = 0.0):
         p, n = self._lists(sel, rows)
-        heads, ldo = self._heads(q), self._rows2d("out", out, rows)
-        if self._heads(out) != heads:
+        pq, ldq, width = self._packed("q", q, rows)
+        po, ldo, wide = self._packed("out", out, rows)
+        if wide != width:
             _refuse(f"out has shape {tuple(out.shape)}, q {tuple(q.shape)}")
-        self._check(self._attend(self.ops.ctx, self.ref, rows.ref, q.data_ptr(), self._rows2d("q", q, rows), heads, scale, softcap, p, n, out.data_ptr(), ldo))
+        st = self._attend(self.ops.ctx, self.ref, rows.ref, pq, ldq, self._heads("q", width), scale, softcap, p, n, po, ldo)
+        if st:
+            self._raise(st)

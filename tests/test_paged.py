@@ -161,20 +161,18 @@ class Array:
             n *= s
         self._dense, self._stride, self._n = tuple(dense), tuple(stride or dense), n
 
+    def get_device(self):
+        return self.device.index
+
     def stride(self):
         return self._stride
 
     def is_contiguous(self):
         return self._stride == self._dense
 
-    def numel(self):
-        return self._n
-
     def data_ptr(self):
         return A
 
-    def __getitem__(self, i):
-        return Array((min(1, self.shape[0]),) + self.shape[1:], self.dtype)
 
 
 class FakeOps:
@@ -234,10 +232,15 @@ def test_views_refuse_calls_that_do_not_fit(lib, host):
     _raises(bad, c.plan, i32(2), Array((2,), "torch.int64"), r)
     _raises(bad, c.plan, i32(2), i32(2), PagedRows(i32(3), i32(3)))
     kv, q, sel, out = Array((3, 2, 64)), Array((3, 8, 64)), i32(3, 2, 4), Array((3, 512))
-    for k, v in ((Array((4, 2, 64)), kv), (Array((3, 128), "torch.float16"), kv), (Array((3, 1, 64)), Array((3, 1, 64))), (kv, Array((3, 128))),
+    for k, v in ((Array((4, 2, 64)), kv), (Array((3, 128), "torch.float16"), kv), (Array((3, 1, 64)), Array((3, 1, 64))), (kv, Array((3, 64))), (kv, Array((3,))),
                  (Array((3, 2, 64), stride=(256, 128, 1)), kv), (Array((3, 2, 64), stride=(128, 64, 2)), kv), (Array((3, 2, 64), device=1), kv)):
         _raises(bad, c.append, r, k, v)
     _raises(bad, c.append, PagedRows(i32(3), i32(3)), kv, kv)
+    away = PagedRows(*(i32(3, device=1) for _ in range(3)))
+    _raises(bad, c.append, away, kv, kv)
+    _raises(bad, c.select, away, q, sel)
+    _raises(bad, c.attend, away, q, sel, out)
+    _raises(bad, PagedRows, i32(3, device=-1), i32(3, device=-1))
     for f in (lambda q, s, o=out: c.select(r, q, s), lambda q, s, o=out: c.attend(r, q, s, o)):
         _raises(bad, f, Array((3, 8, 60)), sel)
         _raises(bad, f, Array((2, 8, 64)), sel)
@@ -257,5 +260,9 @@ def test_views_refuse_calls_that_do_not_fit(lib, host):
     _raises(bad, plan_only.select, r, q, i32(3, 0, 4))
     _raises(bad, _view(lib, host, key_bounds=None).select, r, q, sel)
     _raises(bad, _view(lib, host, k_pool=None, v_pool=None).attend, r, q, sel, out)
+    _raises(abi.CUDA_ERROR, c.append, r, kv, Array((3, 128)))
     _raises(abi.CUDA_ERROR, c.append, r, Array((3, 128), stride=(640, 1)), Array((3, 128), stride=(640, 1)))
     _raises(bad, c.append, r, Array((3, 128), stride=(642, 1)), Array((3, 128), stride=(640, 1)))
+    _raises(bad, c.append, r, kv, Array((3, 2, 64), stride=(64, 64, 1)))
+    _raises(bad, c.select, r, q, Array((3,), "torch.int32"))
+    _raises(bad, c.attend, PagedRows(i32(2), i32(2)), q, i32(2, 2, 4), out)
