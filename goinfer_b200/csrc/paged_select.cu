@@ -17,20 +17,22 @@
 // 2E above (below) that is in (out) for certain; only the blocks between (a handful) are scored in f64. An infinity or a
 // NaN anywhere makes E infinite, and every block is scored in f64.
 //
-// One cluster of CTAs per (row, kv head): the CTAs share out the blocks and send s~ to the first CTA's shared memory, which
-// selects: a histogram of the scores' range in 2048 bins finds the bin of the m-th (and is taken again inside the bin
-// while that is wider than E), and one ordered pass writes the list.
+// One cluster of CTAs per (row, kv head). Each CTA scores a run of the blocks, keeps its s~ in shared memory and decides about
+// its own blocks; what the cluster has to agree on goes through distributed shared memory, every CTA reading the same: the
+// range of s~ and E, a histogram in 512 bins that finds the bin of the m-th (taken again inside the bin while that is wider
+// than 4E), the f64 scores of the blocks in doubt, and how many blocks the CTAs before take. A bit per block says which are
+// in; an ordered pass over the words of bits writes the list.
 #include "paged.cuh"
 
 namespace {
 
 constexpr int kSelThreads = 128, kSelWarps = kSelThreads / 32;
-constexpr int kSelMaxBlocks = 24576;  // 8 bytes a block in the first CTA's shared memory
+constexpr int kSelMaxBlocks = 24576;  // a CTA that is alone holds a score and two bits for each in shared memory
 constexpr int kSelMaxList = 2048;
-constexpr int kSelBins = 2048;
+constexpr int kSelBins = 512;        // four a thread
 constexpr int kSelDoubt = 256;        // blocks in doubt that are ranked in a list; more are selected among in place
 constexpr int kSelMaxCluster = 8;
-constexpr unsigned long long kSelIn = ~0ull, kSelOut = 0ull;  // no score has these keys
+constexpr int kSelRun = 16 * kSelWarps;  // blocks a CTA scores at a time
 
 __device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -47,20 +49,6 @@ __device__ __forceinline__ unsigned half2_bits(float x, float y) {
 __device__ __forceinline__ unsigned long long key_of(double s) {
     const long long b = __double_as_longlong(s);
     return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | 0x8000000000000000ull;
-}
-
-// f over the values of all threads; two barriers, and one more before `red` may be used again
-template <typename T, typename F>
-__device__ __forceinline__ T block_fold(T v, T* red, F f) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    T t = red[0];
-#pragma unroll
-    for (int w = 1; w < kSelWarps; w++) t = f(t, red[w]);
-    return t;
 }
 
 // exclusive scan over the block's threads; total in `total`
@@ -85,25 +73,35 @@ __device__ __forceinline__ int block_scan(int v, int* red, int& total) {
     return before + s - v;
 }
 
-// The thread's bins (top first) hold `hist`; finds the bin in which the running count from the top reaches `need`.
-__device__ __forceinline__ void find_bin(const unsigned* hist, int need, int* red, int* s_bin, int* s_above, int* s_in) {
-    constexpr int BPT = kSelBins / kSelThreads;
-    const int first = kSelBins - 1 - (int)threadIdx.x * BPT;
-    int mine = 0;
-#pragma unroll
-    for (int j = 0; j < BPT; j++) mine += (int)hist[first - j];
+// Finds the bin in which the running count from the top of the cluster's histogram (the sum of the CTAs') reaches `need`.
+// A thread holds four bins.
+__device__ __forceinline__ void find_bin(const unsigned* hist, int ctas, int need, int* red, int* s_bin, int* s_above, int* s_in) {
+    static_assert(kSelBins == 4 * kSelThreads, "four bins a thread");
+    const int first = kSelBins - 4 - 4 * (int)threadIdx.x;
+    uint4 h = make_uint4(0, 0, 0, 0);
+    if (ctas == 1) {
+        h = *reinterpret_cast<const uint4*>(hist + first);
+    } else {
+        for (int w = 0; w < ctas; w++) {
+            const uint4 t = cluster_load_u32x4(cluster_addr(hist + first, w));
+            h.x += t.x; h.y += t.y; h.z += t.z; h.w += t.w;
+        }
+    }
+    const int count[4] = {(int)h.w, (int)h.z, (int)h.y, (int)h.x};
+    const int mine = count[0] + count[1] + count[2] + count[3];
     int total;
     int above = block_scan(mine, red, total);
     if (above < need && above + mine >= need) {
-        for (int j = 0; j < BPT; j++) {
-            const int here = (int)hist[first - j];
-            if (above + here >= need) {
-                *s_bin = first - j;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (above < need && above + count[j] >= need) {
+                *s_bin = first + 3 - j;
                 *s_above = above;
-                *s_in = here;
-                break;
+                *s_in = count[j];
+                above = need;  // found
+            } else {
+                above += count[j];
             }
-            above += here;
         }
     }
     __syncthreads();
@@ -145,15 +143,21 @@ __device__ __forceinline__ double exact_score(const b200_paged_cache& c, int pag
 template <int HD>
 __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_paged_cache c, const int32_t* __restrict__ row_slot,
                                                                    const int32_t* __restrict__ row_pos, const float* __restrict__ q, size_t ldq, int G,
-                                                                   int n_first, int n_recent, int n_select, int32_t* __restrict__ sel) {
-    // first CTA, per middle block: s~ (low word) until the blocks are told apart, then kSelIn, kSelOut or an f64 key
-    extern __shared__ __align__(16) unsigned long long sel_slot[];
-    __shared__ unsigned hist[kSelBins];
-    __shared__ float s_err[kSelMaxCluster * kSelWarps];
-    __shared__ float red_f[kSelWarps];
-    __shared__ int red_i[kSelWarps];
-    __shared__ unsigned long long red_u[kSelWarps], doubt_key[kSelDoubt];
+                                                                   int n_first, int n_recent, int n_select, int max_chunk, int32_t* __restrict__ sel) {
+    // the CTA's blocks: s~ (with many blocks in doubt, words of their keys), a bit for those that are in, one for those in doubt
+    extern __shared__ __align__(16) float sel_score[];
+    unsigned* in_bits = reinterpret_cast<unsigned*>(sel_score + max_chunk);
+    unsigned* doubt_bits = in_bits + max_chunk / 32;
+    __shared__ __align__(16) unsigned hist[kSelBins];
+    __shared__ __align__(16) uint4 q_frag[HD / 32][4][32];  // chunk of dims, part (q > 0 hi, lo; q <= 0 hi, lo), lane
+    // what the CTAs tell one another, by rank (and warp)
+    __shared__ float s_err[kSelMaxCluster * kSelWarps], s_min[kSelMaxCluster * kSelWarps], s_max[kSelMaxCluster * kSelWarps];
+    __shared__ unsigned s_word[kSelMaxCluster * kSelWarps], s_top[kSelMaxCluster * kSelWarps];
+    __shared__ int n_in[kSelMaxCluster], n_doubt_of[kSelMaxCluster], n_left[kSelMaxCluster], n_taken[kSelMaxCluster];
+    __shared__ unsigned long long doubt_key[kSelDoubt];  // the cluster's blocks in doubt: score and block
     __shared__ int doubt[kSelDoubt];
+    __shared__ int own_doubt[kSelDoubt];
+    __shared__ int red_i[kSelWarps];
     __shared__ int s_bin, s_above, s_in, s_doubt;
     const int ctas = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = blockIdx.x / ctas, kvh = blockIdx.y;
@@ -168,27 +172,46 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
     }
     const int n = have - n_first - n_recent;  // the middle blocks n_first .. n_first + n - 1
     const int m = n_select - n_first - n_recent;
-    const int32_t* tbl = c.block_table + (size_t)slot * c.max_blocks + n_first;
+    const int32_t* tbl = c.block_table + (size_t)slot * c.max_blocks + n_first;  // of this CTA's blocks from below on
     const float* qr = q + (size_t)r * ldq + (size_t)kvh * G * HD;
-    cluster_sync();  // the first CTA has started: its shared memory may be written
-    if (m > 0) {
+    if (rank == 0) {
+        for (int i = tid; i < n_first; i += kSelThreads) out[i] = i;
+        for (int i = tid; i < n_recent; i += kSelThreads) out[n_select - n_recent + i] = have - n_recent + i;
+    }
+    if (m <= 0) return;
+    auto everyone = [&] {
+        if (ctas > 1) cluster_sync(); else __syncthreads();
+    };
+    auto tell = [&](auto* what, auto v) {  // a warp's first lanes: one CTA each
+        if (lane < ctas) cluster_store(cluster_addr(what, lane), v);
+    };
+    if (ctas > 1) cluster_sync();  // the CTAs have started: their shared memory may be written
+    // this CTA's blocks: from .. from + own - 1 of the middle, 16 a warp at a time
+    const int chunk = (n + kSelRun * ctas - 1) / (kSelRun * ctas) * kSelRun, from = min(n, rank * chunk), own = min(n, from + chunk) - from;
+    tbl += from;
+    {
         // Fragments: row of A = block, column of B = head. A lane's words of a 16-byte chunk are taken as the dims of its
         // places in the k steps; q is laid out by the same rule, so a bound is loaded as it lies.
         constexpr int CH = HD / 32;  // 16-byte chunks of a row per lane: chunks tig, tig + 4, ...
         const int gid = lane >> 2, tig = lane & 3;
-        unsigned ph[CH][4], nh[CH][4], pl[CH][4], nl[CH][4];  // q > 0 and q <= 0, parts hi and lo; word j: dims 2j, 2j + 1
+        int b0 = 16 * warp;
+        auto page_of = [&](int b) { return b < own ? tbl[b] : 0; };
+        int page0 = page_of(b0 + gid), page1 = page_of(b0 + 8 + gid);
         float f0, f1;  // the columns' powers of two against the group's largest
         {
+            // each warp lays out one chunk of the dims; word j of a part: dims 2j, 2j + 1 of the lane's eight
             const float* qp = qr + (size_t)(gid < G ? gid : 0) * HD + 8 * tig;
-            float4 x[CH][2];
-            float most = 0.f;
+            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, most = 0.f;
 #pragma unroll
-            for (int i = 0; i < CH; i++)
+            for (int i = 0; i < CH; i++) {
+                const float4 u = *reinterpret_cast<const float4*>(qp + 32 * i), v = *reinterpret_cast<const float4*>(qp + 32 * i + 4);
+                const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    x[i][h] = *reinterpret_cast<const float4*>(qp + 32 * i + 4 * h);
-                    most = fmaxf(fmaxf(most, fmaxf(fabsf(x[i][h].x), fabsf(x[i][h].y))), fmaxf(fabsf(x[i][h].z), fabsf(x[i][h].w)));
+                for (int d = 0; d < 8; d++) {
+                    most = fmaxf(most, fabsf(y[d]));
+                    x[d] = i == warp ? y[d] : x[d];
                 }
+            }
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
             // the head's largest |q| comes to [1, 2); 2^-126 and less count as 2^-126 (the floor of E covers them)
@@ -205,24 +228,22 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
                 const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&hi));
                 lo = half2_bits((a - t.x) * 2048.f, (b - t.y) * 2048.f);
             };
-#pragma unroll
-            for (int i = 0; i < CH; i++)
+            if (warp < CH) {
+                unsigned w[4][4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const float4 v = x[i][j >> 1];
-                    const float a = ((j & 1) ? v.z : v.x) * down0 * down1, b = ((j & 1) ? v.w : v.y) * down0 * down1;
+                    const float a = x[2 * j] * down0 * down1, b = x[2 * j + 1] * down0 * down1;
                     // !(q > 0) goes with the lower bounds, a NaN as well
-                    split(a > 0.f ? a : 0.f, b > 0.f ? b : 0.f, ph[i][j], pl[i][j]);
-                    split(a > 0.f ? 0.f : a, b > 0.f ? 0.f : b, nh[i][j], nl[i][j]);
+                    split(a > 0.f ? a : 0.f, b > 0.f ? b : 0.f, w[0][j], w[1][j]);
+                    split(a > 0.f ? 0.f : a, b > 0.f ? 0.f : b, w[2][j], w[3][j]);
                 }
+#pragma unroll
+                for (int t = 0; t < 4; t++) q_frag[warp][t][lane] = make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]);
+            }
         }
-        const unsigned slots0 = cluster_addr(sel_slot, 0);
-        float err = 0.f;
-        const int step = 16 * kSelWarps * ctas;
-        int b0 = 16 * (rank * kSelWarps + warp);
-        auto page_of = [&](int b) { return b < n ? tbl[b] : 0; };
-        int page0 = page_of(b0 + gid), page1 = page_of(b0 + 8 + gid);
-        for (; b0 < n; b0 += step) {
+        __syncthreads();
+        float err = 0.f, mn = INFINITY, mx = -INFINITY;
+        for (; b0 < own; b0 += kSelRun) {
             const bool ok0 = paged_block_ok(page0, c.n_blocks), ok1 = paged_block_ok(page1, c.n_blocks);
             const size_t head = (size_t)c.n_kv_heads, bytes = 4 * HD;
             const uint8_t* p0 = static_cast<const uint8_t*>(c.key_bounds) + ((size_t)(ok0 ? page0 : 0) * head + kvh) * bytes + 16 * tig;
@@ -236,28 +257,23 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
                 l1[i] = ok1 ? __ldg(reinterpret_cast<const uint4*>(p1 + 64 * i)) : z;
                 h1[i] = ok1 ? __ldg(reinterpret_cast<const uint4*>(p1 + 2 * HD + 64 * i)) : z;
             }
-            page0 = page_of(b0 + step + gid);
-            page1 = page_of(b0 + step + 8 + gid);
+            page0 = page_of(b0 + kSelRun + gid);
+            page1 = page_of(b0 + kSelRun + 8 + gid);
             float hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0}, up[4] = {0, 0, 0, 0}, dn[4] = {0, 0, 0, 0};
-            auto two = [&](const uint4& a, const uint4& b, int i, int j, bool upper) {  // words j and j + 1 of a chunk: one k step
-                const unsigned a0 = j ? a.z : a.x, a1 = j ? b.z : b.x, a2 = j ? a.w : a.y, a3 = j ? b.w : b.y;
-                constexpr unsigned abs2 = 0x7fff7fffu;
-                if (upper) {
-                    mma16816(hi, a0, a1, a2, a3, ph[i][j], ph[i][j + 1]);
-                    mma16816(lo, a0, a1, a2, a3, pl[i][j], pl[i][j + 1]);
-                    mma16816(up, a0 & abs2, a1 & abs2, a2 & abs2, a3 & abs2, ph[i][j], ph[i][j + 1]);
-                } else {
-                    mma16816(hi, a0, a1, a2, a3, nh[i][j], nh[i][j + 1]);
-                    mma16816(lo, a0, a1, a2, a3, nl[i][j], nl[i][j + 1]);
-                    mma16816(dn, a0 & abs2, a1 & abs2, a2 & abs2, a3 & abs2, nh[i][j], nh[i][j + 1]);
-                }
+            constexpr unsigned abs2 = 0x7fff7fffu;
+            // two k steps on a chunk of the bounds: words 0, 1 and words 2, 3
+            auto chunk = [&](const uint4& a, const uint4& b, const uint4& qh, const uint4& ql, float (&sum)[4]) {
+                mma16816(hi, a.x, b.x, a.y, b.y, qh.x, qh.y);
+                mma16816(lo, a.x, b.x, a.y, b.y, ql.x, ql.y);
+                mma16816(sum, a.x & abs2, b.x & abs2, a.y & abs2, b.y & abs2, qh.x, qh.y);
+                mma16816(hi, a.z, b.z, a.w, b.w, qh.z, qh.w);
+                mma16816(lo, a.z, b.z, a.w, b.w, ql.z, ql.w);
+                mma16816(sum, a.z & abs2, b.z & abs2, a.w & abs2, b.w & abs2, qh.z, qh.w);
             };
 #pragma unroll
             for (int i = 0; i < CH; i++) {
-                two(h0[i], h1[i], i, 0, true);
-                two(l0[i], l1[i], i, 0, false);
-                two(h0[i], h1[i], i, 2, true);
-                two(l0[i], l1[i], i, 2, false);
+                chunk(h0[i], h1[i], q_frag[i][0][lane], q_frag[i][1][lane], up);
+                chunk(l0[i], l1[i], q_frag[i][2][lane], q_frag[i][3][lane], dn);
             }
             // columns 2 tig and 2 tig + 1 of rows gid (values 0, 1) and gid + 8 (values 2, 3)
             float s[2], E[2];
@@ -277,166 +293,231 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
                     E[h] = fmaxf(E[h], __shfl_xor_sync(0xffffffffu, E[h], o));
                 }
             }
-            if (ok0) err = fmaxf(err, E[0]);
-            if (ok1) err = fmaxf(err, E[1]);
-            if (tig == 0 && b0 + gid < n) cluster_store_u64(slots0 + 8u * (unsigned)(b0 + gid), __float_as_uint(ok0 ? s[0] : -INFINITY));
-            if (tig == 0 && b0 + 8 + gid < n) cluster_store_u64(slots0 + 8u * (unsigned)(b0 + 8 + gid), __float_as_uint(ok1 ? s[1] : -INFINITY));
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const bool ok = h ? ok1 : ok0;
+                const int b = b0 + 8 * h + gid;
+                if (ok) {
+                    err = fmaxf(err, E[h]);
+                    mn = fminf(mn, s[h]);
+                    mx = fmaxf(mx, s[h]);
+                }
+                if (tig == 0 && b < own) sel_score[b] = ok ? s[h] : -INFINITY;
+            }
         }
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, o));
-        if (lane == 0) cluster_store_f32(cluster_addr(s_err + rank * kSelWarps + warp, 0), err);
-    }
-    cluster_sync();  // the scores are in the first CTA's shared memory
-    if (rank != 0) return;
-
-    for (int i = tid; i < n_first; i += kSelThreads) out[i] = i;
-    for (int i = tid; i < n_recent; i += kSelThreads) out[n_select - n_recent + i] = have - n_recent + i;
-    if (m <= 0) return;
-    float err = 0.f;
-    for (int i = 0; i < ctas * kSelWarps; i++) err = fmaxf(err, s_err[i]);
-    err *= 1.01f;  // what the comparisons below round
-    auto approx = [&](int i) { return __uint_as_float((unsigned)sel_slot[i]); };
-    auto least = [](float a, float b) { return fminf(a, b); };
-    auto most = [](float a, float b) { return fmaxf(a, b); };
-
-    // [lo, hi]: holds the m-th largest s~. Unmapped blocks count as the least s~: too much, but never enough to be in for certain.
-    float lo = -INFINITY, hi = INFINITY, floor_s = 0.f;
-    if (err < INFINITY) {
-        float mn = INFINITY, mx = -INFINITY;
-        for (int i = tid; i < n; i += kSelThreads) {
-            const float s = approx(i);
-            if (s > -INFINITY) { mn = fminf(mn, s); mx = fmaxf(mx, s); }
+        for (int o = 4; o < 32; o <<= 1) {
+            err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, o));
+            mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         }
-        lo = block_fold(mn, red_f, least);
-        hi = block_fold(mx, red_f, most);
-        if (!(lo <= hi)) lo = hi = 0.f;  // nothing is mapped
-        floor_s = lo;
+        const int at = rank * kSelWarps + warp;
+        tell(s_err + at, err);
+        tell(s_min + at, mn);
+        tell(s_max + at, mx);
+    }
+    everyone();
+
+    const int told = ctas * kSelWarps;
+    float err = 0.f, lo = INFINITY, hi = -INFINITY;
+    for (int i = 0; i < told; i++) {
+        err = fmaxf(err, s_err[i]);
+        lo = fminf(lo, s_min[i]);
+        hi = fmaxf(hi, s_max[i]);
+    }
+    err *= 1.01f;  // what the comparisons below round
+    // [lo, hi] holds the m-th largest s~. Unmapped blocks count as the least s~: too much, but never enough to be in for certain.
+    if (!(lo <= hi)) lo = hi = 0.f;  // nothing is mapped
+    const float floor_s = lo;
+    auto score = [&](int i) { return fmaxf(sel_score[i], floor_s); };
+    if (err < INFINITY) {
         int need = m;
-        for (int pass = 0; pass < 3 && hi - lo > err; pass++) {
+        for (int pass = 0; pass < 3 && hi - lo > 4.f * err; pass++) {
             const float inv = (float)(kSelBins - 1) / (hi - lo);
+            auto bin_of = [&](float s) { return min(kSelBins - 1, (int)((s - lo) * inv)); };
             for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
             __syncthreads();
-            for (int i = tid; i < n; i += kSelThreads) {
-                const float s = fmaxf(approx(i), floor_s);
-                if (s >= lo && s <= hi) atomicAdd(&hist[min(kSelBins - 1, (int)((s - lo) * inv))], 1u);
+#pragma unroll 4
+            for (int i = tid; i < own; i += kSelThreads) {
+                const float s = score(i);
+                if (s >= lo && s <= hi) atomicAdd(&hist[bin_of(s)], 1u);
             }
-            __syncthreads();
-            find_bin(hist, need, red_i, &s_bin, &s_above, &s_in);
+            everyone();
+            find_bin(hist, ctas, need, red_i, &s_bin, &s_above, &s_in);
             const int bin = s_bin, above = s_above, here = s_in;
-            mn = INFINITY;
-            mx = -INFINITY;
-            for (int i = tid; i < n; i += kSelThreads) {
-                const float s = fmaxf(approx(i), floor_s);
-                if (s >= lo && s <= hi && min(kSelBins - 1, (int)((s - lo) * inv)) == bin) { mn = fminf(mn, s); mx = fmaxf(mx, s); }
+            float mn = INFINITY, mx = -INFINITY;
+#pragma unroll 4
+            for (int i = tid; i < own; i += kSelThreads) {
+                const float s = score(i);
+                if (s >= lo && s <= hi && bin_of(s) == bin) { mn = fminf(mn, s); mx = fmaxf(mx, s); }
             }
-            lo = block_fold(mn, red_f, least);
-            hi = block_fold(mx, red_f, most);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            }
+            tell(s_min + rank * kSelWarps + warp, mn);
+            tell(s_max + rank * kSelWarps + warp, mx);
+            everyone();
+            lo = INFINITY;
+            hi = -INFINITY;
+            for (int i = 0; i < told; i++) {
+                lo = fminf(lo, s_min[i]);
+                hi = fmaxf(hi, s_max[i]);
+            }
             need -= above;
             if (need == here) hi = lo;       // the m-th is the bin's least
             else if (need == 1) lo = hi;     // ... or its largest
         }
+    } else {
+        lo = -INFINITY;
+        hi = INFINITY;
     }
     // in for certain, out for certain, in doubt
     const float sure_in = hi + 2.f * err, sure_out = lo - 2.f * err;
     if (tid == 0) s_doubt = 0;
     __syncthreads();
+    const int words = (own + 31) >> 5;
     int in = 0;
-    for (int i = tid; i < n; i += kSelThreads) {
-        const float s = fmaxf(approx(i), floor_s);
-        if (s > sure_in) {
-            in++;
-            sel_slot[i] = kSelIn;
-        } else if (s < sure_out) {
-            sel_slot[i] = kSelOut;
-        } else {
-            const int at = atomicAdd(&s_doubt, 1);
-            if (at < kSelDoubt) doubt[at] = i;
-            sel_slot[i] = 1;  // in doubt: no f64 score has this key
+#pragma unroll 2
+    for (int w = warp; w < words; w += kSelWarps) {
+        const int i = 32 * w + lane;
+        const float s = i < own ? score(i) : -INFINITY;
+        const bool is_in = i < own && s > sure_in, is_doubt = i < own && !(s > sure_in) && !(s < sure_out);
+        const unsigned in_word = __ballot_sync(0xffffffffu, is_in), doubt_word = __ballot_sync(0xffffffffu, is_doubt);
+        if (doubt_word) {
+            int at = lane == 0 ? atomicAdd(&s_doubt, __popc(doubt_word)) : 0;
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(doubt_word & ((1u << lane) - 1u));
+            if (is_doubt && at < kSelDoubt) own_doubt[at] = i;
         }
+        if (lane == 0) {
+            in_bits[w] = in_word;
+            doubt_bits[w] = doubt_word;
+        }
+        in += __popc(in_word);
     }
-    in = block_fold(in, red_i, [](int a, int b) { return a + b; });
-    const int n_doubt = s_doubt;
-    int need = m - in;  // 1 .. n_doubt of those in doubt
-    unsigned long long kmin = kSelIn, kmax = kSelIn;  // the list: keys above kmax, and the first `need` from kmin to kmax
+    if (lane == 0) red_i[warp] = in;
+    __syncthreads();
+    const int n_own = s_doubt;  // this CTA's blocks in doubt
+    if (warp == 0) {
+        in = 0;
+        for (int w = 0; w < kSelWarps; w++) in += red_i[w];
+        tell(n_in + rank, in);
+        tell(n_doubt_of + rank, n_own);
+    }
+    everyone();
+    int need = m, n_doubt = 0, before = 0;  // before: blocks in doubt of the CTAs ahead
+    for (int w = 0; w < ctas; w++) {
+        if (w == rank) before = n_doubt;
+        need -= n_in[w];
+        n_doubt += n_doubt_of[w];
+    }
+    // `need`, 1 .. n_doubt, of those in doubt are in
     constexpr int LPB = HD / 8, BPW = 32 / LPB;
     const int sub = lane % LPB, part = lane / LPB;
     if (n_doubt == need) {
-        kmin = 1;
-        need = m;
+        for (int w = tid; w < words; w += kSelThreads) in_bits[w] |= doubt_bits[w];
     } else if (n_doubt <= kSelDoubt) {
-        for (int j0 = warp * BPW; j0 < n_doubt; j0 += kSelWarps * BPW) {
-            const int j = j0 + part;
-            const double s = exact_score<HD>(c, j < n_doubt ? tbl[doubt[j]] : 0, kvh, qr, G, sub);
-            if (sub == 0 && j < n_doubt) doubt_key[j] = key_of(s);
+        for (int j0 = warp * BPW; j0 < n_own; j0 += kSelWarps * BPW) {
+            const int j = j0 + part, i = j < n_own ? own_doubt[j] : 0;
+            const unsigned long long k = key_of(exact_score<HD>(c, j < n_own ? tbl[i] : 0, kvh, qr, G, sub));
+            if (j < n_own && sub < ctas) {  // (a cluster has at most as many CTAs as a block has lanes)
+                cluster_store(cluster_addr(doubt_key + before + j, sub), k);
+                cluster_store(cluster_addr(doubt + before + j, sub), from + i);
+            }
         }
-        __syncthreads();
-        for (int j = tid; j < n_doubt; j += kSelThreads) {
-            const unsigned long long k = doubt_key[j];
-            const int i = doubt[j];
-            int before = 0;
-            for (int t = 0; t < n_doubt; t++) before += doubt_key[t] > k || (doubt_key[t] == k && doubt[t] < i);
-            sel_slot[i] = before < need ? kSelIn : kSelOut;
+        everyone();
+        for (int j = tid; j < n_own; j += kSelThreads) {
+            const unsigned long long k = doubt_key[before + j];
+            const int i = own_doubt[j];
+            int higher = 0;
+            for (int t = 0; t < n_doubt; t++) higher += doubt_key[t] > k || (doubt_key[t] == k && doubt[t] < from + i);
+            if (higher < need) atomicOr(&in_bits[i >> 5], 1u << (i & 31));
         }
-        need = m;
     } else {
-        __syncthreads();
-        for (int i0 = warp * BPW; i0 < n; i0 += kSelWarps * BPW) {
-            const int i = i0 + part;
-            const bool here = i < n && sel_slot[i] == 1;
-            if (!__any_sync(0xffffffffu, here)) continue;
-            const double s = exact_score<HD>(c, here ? tbl[i] : 0, kvh, qr, G, sub);
-            __syncwarp();
-            if (sub == 0 && here) sel_slot[i] = key_of(s);
-        }
-        __syncthreads();
-        kmin = kSelIn;
-        kmax = kSelOut;
-        for (int i = tid; i < n; i += kSelThreads) {
-            const unsigned long long k = sel_slot[i];
-            if (k != kSelIn && k != kSelOut) {
-                kmin = min(kmin, k);
-                kmax = max(kmax, k);
+        // Equal scores by the hundred, or an infinite E: the upper words of the f64 keys are selected among first, then the
+        // lower words of those whose upper word is the last one taken, then the blocks' order decides.
+        unsigned* key = reinterpret_cast<unsigned*>(sel_score);
+        auto in_doubt = [&](int i) { return ((doubt_bits[i >> 5] >> (i & 31)) & 1u) != 0; };
+        for (int level = 0; level < 2 && need > 0; level++) {
+            __syncthreads();
+            unsigned kmin = ~0u, kmax = 0u;
+            for (int i0 = warp * BPW; i0 < own; i0 += kSelWarps * BPW) {
+                const int i = i0 + part;
+                const bool here = i < own && in_doubt(i);
+                if (!__any_sync(0xffffffffu, here)) continue;
+                const unsigned long long k = key_of(exact_score<HD>(c, here ? tbl[i] : 0, kvh, qr, G, sub));
+                const unsigned word = level == 0 ? (unsigned)(k >> 32) : (unsigned)k;
+                if (here) {
+                    if (sub == 0) key[i] = word;
+                    kmin = min(kmin, word);
+                    kmax = max(kmax, word);
+                }
             }
-        }
-        kmin = block_fold(kmin, red_u, [](unsigned long long a, unsigned long long b) { return a < b ? a : b; });
-        kmax = block_fold(kmax, red_u, [](unsigned long long a, unsigned long long b) { return a < b ? b : a; });
-        while (true) {  // at most six divisions of a 64-bit range by 2048
-            const int width = 64 - __clzll((long long)(kmax - kmin));
-            const int shift = width > 11 ? width - 11 : 0;
-            __syncthreads();
-            for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
-            __syncthreads();
-            for (int i = tid; i < n; i += kSelThreads) {
-                const unsigned long long k = sel_slot[i];
-                if (k >= kmin && k <= kmax) atomicAdd(&hist[(unsigned)((k - kmin) >> shift)], 1u);
+            tell(s_word + rank * kSelWarps + warp, __reduce_min_sync(0xffffffffu, kmin));
+            tell(s_top + rank * kSelWarps + warp, __reduce_max_sync(0xffffffffu, kmax));
+            everyone();
+            for (int i = 0; i < told; i++) {
+                kmin = min(kmin, s_word[i]);
+                kmax = max(kmax, s_top[i]);
             }
-            __syncthreads();
-            find_bin(hist, need, red_i, &s_bin, &s_above, &s_in);
-            need -= s_above;
-            const unsigned long long from = kmin + ((unsigned long long)s_bin << shift), to = from + ((1ull << shift) - 1ull);
-            kmax = to < kmax ? to : kmax;
-            kmin = from;
-            if (s_in == need || shift == 0) break;
+            int here;
+            while (true) {  // at most four divisions of the range by 512
+                const int width = 32 - __clz((int)(kmax - kmin)), shift = width > 9 ? width - 9 : 0;
+                for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+                __syncthreads();
+                for (int i = tid; i < own; i += kSelThreads)
+                    if (in_doubt(i) && key[i] >= kmin && key[i] <= kmax) atomicAdd(&hist[(key[i] - kmin) >> shift], 1u);
+                everyone();
+                find_bin(hist, ctas, need, red_i, &s_bin, &s_above, &s_in);
+                here = s_in;
+                need -= s_above;
+                const unsigned first = kmin + ((unsigned)s_bin << shift), width_less_1 = (1u << shift) - 1u;
+                kmax = kmax - first < width_less_1 ? kmax : first + width_less_1;  // (first + width may pass 2^32)
+                kmin = first;
+                everyone();  // the histograms have been read
+                if (here == need || shift == 0) break;
+            }
+            // what lies above is in; what lies between is in when all of it is needed, else in doubt still
+            const bool all = here == need;
+            for (int w = warp; w < words; w += kSelWarps) {
+                const int i = 32 * w + lane;
+                const bool d = i < own && in_doubt(i);
+                const unsigned k = d ? key[i] : 0u;
+                const unsigned edge = __ballot_sync(0xffffffffu, d && k >= kmin && k <= kmax), above = __ballot_sync(0xffffffffu, d && k > kmax);
+                __syncwarp();
+                if (lane == 0) {
+                    in_bits[w] |= above | (all ? edge : 0u);
+                    doubt_bits[w] = edge;
+                }
+            }
+            if (all) need = 0;
         }
+        __syncthreads();
+        int left = 0;
+        for (int w = lane; w < words; w += 32) left += __popc(doubt_bits[w]);
+        left = __reduce_add_sync(0xffffffffu, left);
+        if (warp == 0) tell(n_left + rank, left);
+        everyone();
+        for (int w = 0; w < rank; w++) need -= n_left[w];
+        if (tid == 0)  // the first of equals
+            for (int w = 0; need > 0 && w < words; w++)
+                for (unsigned bits = doubt_bits[w]; bits && need > 0; bits &= bits - 1u, need--) in_bits[w] |= bits & (0u - bits);
     }
     __syncthreads();
-    // an ordered pass over runs of blocks: a run a thread
-    const int per = (n + kSelThreads - 1) / kSelThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
-    int n_above = 0, n_edge = 0;
-    for (int i = i0; i < i1; i++) {
-        n_above += sel_slot[i] > kmax;
-        n_edge += sel_slot[i] >= kmin && sel_slot[i] <= kmax;
-    }
+    // a run of words a thread: its first place in the list by a scan of the counts
+    const int per = (words + kSelThreads - 1) / kSelThreads, w0 = min(words, tid * per), w1 = min(words, w0 + per);
+    int mine = 0;
+    for (int w = w0; w < w1; w++) mine += __popc(in_bits[w]);
     int total;
-    const int above0 = block_scan(n_above, red_i, total);
-    int edge = block_scan(n_edge, red_i, total);
-    int at = n_first + above0 + min(edge, need);
-    for (int i = i0; i < i1; i++) {
-        const unsigned long long k = sel_slot[i];
-        const bool is_edge = k >= kmin && k <= kmax;
-        if (k > kmax || (is_edge && edge < need)) out[at++] = n_first + i;
-        edge += is_edge;
+    int at = n_first + block_scan(mine, red_i, total);
+    if (ctas > 1) {
+        if (warp == 0) tell(n_taken + rank, total);
+        cluster_sync();
+        for (int w = 0; w < rank; w++) at += n_taken[w];
     }
+    for (int w = w0; w < w1; w++)
+        for (unsigned bits = in_bits[w]; bits && at < n_select - n_recent; bits &= bits - 1u) out[at++] = n_first + from + 32 * w + __ffs((int)bits) - 1;
 }
 
 }  // namespace
@@ -465,12 +546,13 @@ extern "C" int b200_paged_select(b200_ctx* ctx, const b200_paged_cache* c, const
     const int G = n_heads / c->n_kv_heads;
     auto kernel = c->head_dim == 128 ? paged_select_kernel<128> : paged_select_kernel<64>;
     static SmemLimit limit[2];
-    const size_t smem = 8 * (size_t)c->max_blocks;
-    CUDA_TRY(ctx, limit[c->head_dim == 128].raise(kernel, ctx->device, 8 * (size_t)kSelMaxBlocks));
     int ctas = 1;
-    while (ctas < 8 && (long long)r->n_rows * c->n_kv_heads * ctas < 2 * ctx->sm_count && c->max_blocks / ctas > 64) ctas *= 2;
-    launch_cluster(kernel, ctas, dim3((unsigned)(r->n_rows * ctas), c->n_kv_heads), dim3(kSelThreads), smem, ctx->stream, *c, r->row_slot, r->row_pos, q,
-                   (size_t)ldq, G, n_first, n_recent, n_select, sel);
+    while (ctas < kSelMaxCluster && (long long)r->n_rows * c->n_kv_heads * ctas < 2 * ctx->sm_count && c->max_blocks > kSelRun * ctas) ctas *= 2;
+    const int chunk = ceil_div(c->max_blocks, kSelRun * ctas) * kSelRun;  // of one CTA
+    auto smem = [](int blocks) { return (size_t)blocks * 4 + 2 * ((size_t)blocks / 8); };
+    CUDA_TRY(ctx, limit[c->head_dim == 128].raise(kernel, ctx->device, smem(kSelMaxBlocks)));
+    launch_cluster(kernel, ctas, dim3((unsigned)(r->n_rows * ctas), c->n_kv_heads), dim3(kSelThreads), smem(chunk), ctx->stream, *c, r->row_slot, r->row_pos, q,
+                   (size_t)ldq, G, n_first, n_recent, n_select, chunk, sel);
     LAUNCH_CHECK(ctx);
     return B200_OK;
 }

@@ -261,11 +261,12 @@ def test_select_takes_the_best_blocks(ops, rows, kv, G, hd, br, max_blocks, n_fi
     np.testing.assert_array_equal(sel.cpu().numpy(), _select_reference(q, bounds, table, slot, pos, br, kv, n_first, n_recent, n, before))
 
 
-def test_select_values_out_of_the_ordinary(ops):
+@pytest.mark.parametrize("max_blocks", [80, 900])
+def test_select_values_out_of_the_ordinary(ops, max_blocks):
     """Zeros of both signs, subnormal and largest fp16 bounds, infinities and NaN in the bounds and in q, bad pages, equal rows,
     positions past the table, and scores that agree to 30 bits."""
     rng = np.random.default_rng(3)
-    rows, kv, G, hd, br, max_blocks, n = 12, 2, 2, 64, 16, 80, 20
+    rows, kv, G, hd, br, n = 12, 2, 2, 64, 16, 20
     n_blocks = 200
     bounds = np.sort(rng.normal(0, 1, (n_blocks, kv, 2, hd)), axis=2).astype(np.float16)
     bounds[1:8] = 0.0
