@@ -19,9 +19,9 @@
 //
 // One cluster of CTAs per (row, kv head). Each CTA scores a run of the blocks, keeps its s~ in shared memory and decides about
 // its own blocks; what the cluster has to agree on goes through distributed shared memory, every CTA reading the same: the
-// range of s~ and E, a histogram in 512 bins that finds the bin of the m-th (taken again inside the bin while that is wider
-// than 4E), the f64 scores of the blocks in doubt, and how many blocks the CTAs before take. A bit per block says which are
-// in; an ordered pass over the words of bits writes the list.
+// range of s~ and E, a histogram in 512 bins that finds the bin of the m-th (taken again inside the bin where that is much
+// wider than E), and the f64 scores of the blocks in doubt. A bit per block says which are in; an ordered pass over the
+// words of bits writes the list.
 #include "paged.cuh"
 
 namespace {
@@ -107,10 +107,10 @@ __device__ __forceinline__ void find_bin(const unsigned* hist, int ctas, int nee
     __syncthreads();
 }
 
-// f64 score of one block by the HD/8 lanes that share it (eight dims each, `sub` among them); every lane gets it. The
-// bounds' order of summation is the same for every block, so equal bounds have equal scores.
+// Key of the f64 score of one block by the HD/8 lanes that share it (eight dims each, `sub` among them); every lane gets it.
+// The order of summation is the same for every block, so equal bounds have equal scores.
 template <int HD>
-__device__ __forceinline__ double exact_score(const b200_paged_cache& c, int page, int kvh, const float* q, int G, int sub) {
+__device__ __forceinline__ unsigned long long exact_key(const b200_paged_cache& c, int page, int kvh, const float* q, int G, int sub) {
     constexpr int LPB = HD / 8;
     constexpr double top = 1.7976931348623157e308;
     const bool ok = paged_block_ok(page, c.n_blocks);
@@ -124,20 +124,24 @@ __device__ __forceinline__ double exact_score(const b200_paged_cache& c, int pag
     const __half* hh = reinterpret_cast<const __half*>(&hi);
     double best = -INFINITY;
     bool nan = false;
+#pragma unroll 4
     for (int g = 0; g < G; g++) {
-        double s = 0.0;
+        const float4 a = *reinterpret_cast<const float4*>(q + g * HD + 8 * sub), b = *reinterpret_cast<const float4*>(q + g * HD + 8 * sub + 4);
+        const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        double s = 0.0, t = 0.0;
 #pragma unroll
-        for (int d = 0; d < 8; d++) {
-            const float x = q[(size_t)g * HD + 8 * sub + d];
-            s = fma((double)x, (double)__half2float(x > 0.f ? hh[d] : lh[d]), s);
+        for (int d = 0; d < 8; d += 2) {
+            s = fma((double)x[d], (double)__half2float(x[d] > 0.f ? hh[d] : lh[d]), s);
+            t = fma((double)x[d + 1], (double)__half2float(x[d + 1] > 0.f ? hh[d + 1] : lh[d + 1]), t);
         }
+        s += t;
 #pragma unroll
         for (int o = LPB / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         nan |= s != s;
         best = fmax(best, s);
     }
     best = nan ? top : fmin(fmax(best, -top), top) + 0.0;  // -0 -> +0
-    return ok ? best : -top;
+    return key_of(ok ? best : -top);
 }
 
 template <int HD>
@@ -149,6 +153,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
     unsigned* in_bits = reinterpret_cast<unsigned*>(sel_score + max_chunk);
     unsigned* doubt_bits = in_bits + max_chunk / 32;
     __shared__ __align__(16) unsigned hist[kSelBins];
+    __shared__ __align__(16) float sq[8][HD];
     __shared__ __align__(16) uint4 q_frag[HD / 32][4][32];  // chunk of dims, part (q > 0 hi, lo; q <= 0 hi, lo), lane
     // what the CTAs tell one another, by rank (and warp)
     __shared__ float s_err[kSelMaxCluster * kSelWarps], s_min[kSelMaxCluster * kSelWarps], s_max[kSelMaxCluster * kSelWarps];
@@ -185,7 +190,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
     auto tell = [&](auto* what, auto v) {  // a warp's first lanes: one CTA each
         if (lane < ctas) cluster_store(cluster_addr(what, lane), v);
     };
-    if (ctas > 1) cluster_sync();  // the CTAs have started: their shared memory may be written
+    if (ctas > 1) cluster_arrive();
     // this CTA's blocks: from .. from + own - 1 of the middle, 16 a warp at a time
     const int chunk = (n + kSelRun * ctas - 1) / (kSelRun * ctas) * kSelRun, from = min(n, rank * chunk), own = min(n, from + chunk) - from;
     tbl += from;
@@ -196,11 +201,13 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
         const int gid = lane >> 2, tig = lane & 3;
         int b0 = 16 * warp;
         auto page_of = [&](int b) { return b < own ? tbl[b] : 0; };
-        int page0 = page_of(b0 + gid), page1 = page_of(b0 + 8 + gid);
+        int page0 = page_of(b0 + gid), page1 = page_of(b0 + 8 + gid), next0 = page_of(b0 + kSelRun + gid), next1 = page_of(b0 + kSelRun + 8 + gid);
+        for (int i = tid; i < G * HD / 4; i += kSelThreads) reinterpret_cast<float4*>(&sq[0][0])[i] = reinterpret_cast<const float4*>(qr)[i];
+        __syncthreads();
         float f0, f1;  // the columns' powers of two against the group's largest
         {
             // each warp lays out one chunk of the dims; word j of a part: dims 2j, 2j + 1 of the lane's eight
-            const float* qp = qr + (size_t)(gid < G ? gid : 0) * HD + 8 * tig;
+            const float* qp = sq[gid < G ? gid : 0] + 8 * tig;
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, most = 0.f;
 #pragma unroll
             for (int i = 0; i < CH; i++) {
@@ -257,8 +264,14 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
                 l1[i] = ok1 ? __ldg(reinterpret_cast<const uint4*>(p1 + 64 * i)) : z;
                 h1[i] = ok1 ? __ldg(reinterpret_cast<const uint4*>(p1 + 2 * HD + 64 * i)) : z;
             }
-            page0 = page_of(b0 + kSelRun + gid);
-            page1 = page_of(b0 + kSelRun + 8 + gid);
+            // the next run's bounds are on their way to L2 (a line a lane), the one's after it pages to registers
+            const size_t line = (size_t)128 * tig;
+            if (line < bytes && paged_block_ok(next0, c.n_blocks)) prefetch_l2(static_cast<const uint8_t*>(c.key_bounds) + ((size_t)next0 * head + kvh) * bytes + line);
+            if (line < bytes && paged_block_ok(next1, c.n_blocks)) prefetch_l2(static_cast<const uint8_t*>(c.key_bounds) + ((size_t)next1 * head + kvh) * bytes + line);
+            page0 = next0;
+            page1 = next1;
+            next0 = page_of(b0 + 2 * kSelRun + gid);
+            next1 = page_of(b0 + 2 * kSelRun + 8 + gid);
             float hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0}, up[4] = {0, 0, 0, 0}, dn[4] = {0, 0, 0, 0};
             constexpr unsigned abs2 = 0x7fff7fffu;
             // two k steps on a chunk of the bounds: words 0, 1 and words 2, 3
@@ -311,6 +324,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
             mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         }
+        if (ctas > 1) cluster_wait();  // the CTAs have started: their shared memory may be written
         const int at = rank * kSelWarps + warp;
         tell(s_err + at, err);
         tell(s_min + at, mn);
@@ -331,43 +345,23 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
     const float floor_s = lo;
     auto score = [&](int i) { return fmaxf(sel_score[i], floor_s); };
     if (err < INFINITY) {
-        int need = m;
-        for (int pass = 0; pass < 3 && hi - lo > 4.f * err; pass++) {
+        for (int pass = 0; pass < 3 && hi - lo > 16.f * err; pass++) {
+            // s~ above the range (from the second pass on) counts in the top bin: the m-th lies in the range, so its bin is found
             const float inv = (float)(kSelBins - 1) / (hi - lo);
-            auto bin_of = [&](float s) { return min(kSelBins - 1, (int)((s - lo) * inv)); };
-            for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+            *reinterpret_cast<uint4*>(hist + 4 * tid) = make_uint4(0, 0, 0, 0);
             __syncthreads();
 #pragma unroll 4
             for (int i = tid; i < own; i += kSelThreads) {
                 const float s = score(i);
-                if (s >= lo && s <= hi) atomicAdd(&hist[bin_of(s)], 1u);
+                if (s >= lo) atomicAdd(&hist[min(kSelBins - 1, (int)((fminf(s, hi) - lo) * inv))], 1u);
             }
             everyone();
-            find_bin(hist, ctas, need, red_i, &s_bin, &s_above, &s_in);
-            const int bin = s_bin, above = s_above, here = s_in;
-            float mn = INFINITY, mx = -INFINITY;
-#pragma unroll 4
-            for (int i = tid; i < own; i += kSelThreads) {
-                const float s = score(i);
-                if (s >= lo && s <= hi && bin_of(s) == bin) { mn = fminf(mn, s); mx = fmaxf(mx, s); }
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            }
-            tell(s_min + rank * kSelWarps + warp, mn);
-            tell(s_max + rank * kSelWarps + warp, mx);
-            everyone();
-            lo = INFINITY;
-            hi = -INFINITY;
-            for (int i = 0; i < told; i++) {
-                lo = fminf(lo, s_min[i]);
-                hi = fmaxf(hi, s_max[i]);
-            }
-            need -= above;
-            if (need == here) hi = lo;       // the m-th is the bin's least
-            else if (need == 1) lo = hi;     // ... or its largest
+            find_bin(hist, ctas, m, red_i, &s_bin, &s_above, &s_in);
+            // the bin's edges, out by more than the index above rounds (2^-22 of the range)
+            const float slack = (hi - lo) * 0x1p-20f, from_s = lo + (float)s_bin / inv - slack, to_s = lo + (float)(s_bin + 1) / inv + slack;
+            lo = fmaxf(lo, from_s);
+            hi = fminf(hi, to_s);
+            if (hi - lo > 16.f * err) everyone();  // the histograms have been read: they may be cleared
         }
     } else {
         lo = -INFINITY;
@@ -407,8 +401,12 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
     }
     everyone();
     int need = m, n_doubt = 0, before = 0;  // before: blocks in doubt of the CTAs ahead
+    int first = n_first;                    // this CTA's first place in the list
     for (int w = 0; w < ctas; w++) {
-        if (w == rank) before = n_doubt;
+        if (w == rank) {
+            before = n_doubt;
+            first += m - need;
+        }
         need -= n_in[w];
         n_doubt += n_doubt_of[w];
     }
@@ -417,23 +415,31 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
     const int sub = lane % LPB, part = lane / LPB;
     if (n_doubt == need) {
         for (int w = tid; w < words; w += kSelThreads) in_bits[w] |= doubt_bits[w];
+        first += before;
     } else if (n_doubt <= kSelDoubt) {
         for (int j0 = warp * BPW; j0 < n_own; j0 += kSelWarps * BPW) {
             const int j = j0 + part, i = j < n_own ? own_doubt[j] : 0;
-            const unsigned long long k = key_of(exact_score<HD>(c, j < n_own ? tbl[i] : 0, kvh, qr, G, sub));
+            const unsigned long long k = exact_key<HD>(c, j < n_own ? tbl[i] : 0, kvh, &sq[0][0], G, sub);
             if (j < n_own && sub < ctas) {  // (a cluster has at most as many CTAs as a block has lanes)
                 cluster_store(cluster_addr(doubt_key + before + j, sub), k);
                 cluster_store(cluster_addr(doubt + before + j, sub), from + i);
             }
         }
         everyone();
-        for (int j = tid; j < n_own; j += kSelThreads) {
-            const unsigned long long k = doubt_key[before + j];
-            const int i = own_doubt[j];
-            int higher = 0;
-            for (int t = 0; t < n_doubt; t++) higher += doubt_key[t] > k || (doubt_key[t] == k && doubt[t] < from + i);
-            if (higher < need) atomicOr(&in_bits[i >> 5], 1u << (i & 31));
+        int ahead = 0;  // of those that the CTAs ahead hold, the ones that are in
+        for (int j0 = 0; j0 < n_doubt; j0 += kSelThreads) {
+            const int j = j0 + tid;
+            int higher = n_doubt;
+            if (j < n_doubt) {
+                const unsigned long long k = doubt_key[j];
+                const int i = doubt[j];
+                higher = 0;
+                for (int t = 0; t < n_doubt; t++) higher += doubt_key[t] > k || (doubt_key[t] == k && doubt[t] < i);
+                if (higher < need && j >= before && j < before + n_own) atomicOr(&in_bits[(i - from) >> 5], 1u << ((i - from) & 31));
+            }
+            ahead += __syncthreads_count(higher < need && j < before);
         }
+        first += ahead;
     } else {
         // Equal scores by the hundred, or an infinite E: the upper words of the f64 keys are selected among first, then the
         // lower words of those whose upper word is the last one taken, then the blocks' order decides.
@@ -446,7 +452,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
                 const int i = i0 + part;
                 const bool here = i < own && in_doubt(i);
                 if (!__any_sync(0xffffffffu, here)) continue;
-                const unsigned long long k = key_of(exact_score<HD>(c, here ? tbl[i] : 0, kvh, qr, G, sub));
+                const unsigned long long k = exact_key<HD>(c, here ? tbl[i] : 0, kvh, &sq[0][0], G, sub);
                 const unsigned word = level == 0 ? (unsigned)(k >> 32) : (unsigned)k;
                 if (here) {
                     if (sub == 0) key[i] = word;
@@ -472,9 +478,9 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
                 find_bin(hist, ctas, need, red_i, &s_bin, &s_above, &s_in);
                 here = s_in;
                 need -= s_above;
-                const unsigned first = kmin + ((unsigned)s_bin << shift), width_less_1 = (1u << shift) - 1u;
-                kmax = kmax - first < width_less_1 ? kmax : first + width_less_1;  // (first + width may pass 2^32)
-                kmin = first;
+                const unsigned edge = kmin + ((unsigned)s_bin << shift), width_less_1 = (1u << shift) - 1u;
+                kmax = kmax - edge < width_less_1 ? kmax : edge + width_less_1;  // (edge + width may pass 2^32)
+                kmin = edge;
                 everyone();  // the histograms have been read
                 if (here == need || shift == 0) break;
             }
@@ -503,21 +509,32 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
         if (tid == 0)  // the first of equals
             for (int w = 0; need > 0 && w < words; w++)
                 for (unsigned bits = doubt_bits[w]; bits && need > 0; bits &= bits - 1u, need--) in_bits[w] |= bits & (0u - bits);
+        __syncthreads();
+        int taken = 0;
+        for (int w = lane; w < words; w += 32) taken += __popc(in_bits[w]);
+        taken = __reduce_add_sync(0xffffffffu, taken);
+        if (warp == 0) tell(n_taken + rank, taken);
+        everyone();
+        first = n_first;
+        for (int w = 0; w < rank; w++) first += n_taken[w];
     }
     __syncthreads();
-    // a run of words a thread: its first place in the list by a scan of the counts
-    const int per = (words + kSelThreads - 1) / kSelThreads, w0 = min(words, tid * per), w1 = min(words, w0 + per);
-    int mine = 0;
-    for (int w = w0; w < w1; w++) mine += __popc(in_bits[w]);
-    int total;
-    int at = n_first + block_scan(mine, red_i, total);
-    if (ctas > 1) {
-        if (warp == 0) tell(n_taken + rank, total);
-        cluster_sync();
-        for (int w = 0; w < rank; w++) at += n_taken[w];
+    // every warp scans the words' counts and writes the blocks of its own words
+    for (int g = 0; g < words; g += 32) {
+        const unsigned mine = g + lane < words ? in_bits[g + lane] : 0u;
+        int end = __popc(mine);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += t;
+        }
+        for (int w = warp; w < 32 && g + w < words; w += kSelWarps) {
+            const unsigned bits = __shfl_sync(0xffffffffu, mine, w);
+            const int at = first + __shfl_sync(0xffffffffu, end, w) - __popc(bits >> lane);
+            if (((bits >> lane) & 1u) && at < n_select - n_recent) out[at] = n_first + from + 32 * (g + w) + lane;
+        }
+        first += __shfl_sync(0xffffffffu, end, 31);
     }
-    for (int w = w0; w < w1; w++)
-        for (unsigned bits = in_bits[w]; bits && at < n_select - n_recent; bits &= bits - 1u) out[at++] = n_first + from + 32 * w + __ffs((int)bits) - 1;
 }
 
 }  // namespace
