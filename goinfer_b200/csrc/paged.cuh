@@ -80,7 +80,6 @@ __device__ __forceinline__ void cluster_sync() {
 // The same barrier in two halves, without an order of memory: behind the wait every CTA of the cluster has started.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 // Address of a shared variable of this CTA in the CTA `rank` of the cluster.
 __device__ __forceinline__ unsigned cluster_addr(const void* p, unsigned rank) {
     unsigned a = (unsigned)__cvta_generic_to_shared(p), r;

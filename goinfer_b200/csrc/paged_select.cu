@@ -39,6 +39,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// A load that stays where it is written: all of a run's loads go out before its first product waits for one.
+__device__ __forceinline__ uint4 load16(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ unsigned half2_bits(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -144,8 +150,10 @@ __device__ __forceinline__ unsigned long long exact_key(const b200_paged_cache& 
     return key_of(ok ? best : -top);
 }
 
+// Four CTAs an SM: the 128 registers this leaves a thread hold a run's bounds (64) on their way; with fewer the compiler starts
+// the products before the last load is out (batch 66 us either way, long contexts 50 against 58 us).
 template <int HD>
-__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_paged_cache c, const int32_t* __restrict__ row_slot,
+__global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200_paged_cache c, const int32_t* __restrict__ row_slot,
                                                                    const int32_t* __restrict__ row_pos, const float* __restrict__ q, size_t ldq, int G,
                                                                    int n_first, int n_recent, int n_select, int max_chunk, int32_t* __restrict__ sel) {
     // the CTA's blocks: s~ (with many blocks in doubt, words of their keys), a bit for those that are in, one for those in doubt
@@ -201,33 +209,28 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
         const int gid = lane >> 2, tig = lane & 3;
         int b0 = 16 * warp;
         auto page_of = [&](int b) { return b < own ? tbl[b] : 0; };
-        int page0 = page_of(b0 + gid), page1 = page_of(b0 + 8 + gid), next0 = page_of(b0 + kSelRun + gid), next1 = page_of(b0 + kSelRun + 8 + gid);
+        int page0 = page_of(b0 + gid), page1 = page_of(b0 + 8 + gid);
         for (int i = tid; i < G * HD / 4; i += kSelThreads) reinterpret_cast<float4*>(&sq[0][0])[i] = reinterpret_cast<const float4*>(qr)[i];
         __syncthreads();
-        float f0, f1;  // the columns' powers of two against the group's largest
+        // the columns' powers of two against the group's largest; columns past the group repeat its first head
+        float f0, f1;
         {
-            // each warp lays out one chunk of the dims; word j of a part: dims 2j, 2j + 1 of the lane's eight
             const float* qp = sq[gid < G ? gid : 0] + 8 * tig;
-            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, most = 0.f;
+            float most = 0.f;
 #pragma unroll
-            for (int i = 0; i < CH; i++) {
-                const float4 u = *reinterpret_cast<const float4*>(qp + 32 * i), v = *reinterpret_cast<const float4*>(qp + 32 * i + 4);
-                const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int d = 0; d < 8; d++) {
-                    most = fmaxf(most, fabsf(y[d]));
-                    x[d] = i == warp ? y[d] : x[d];
-                }
+            for (int i = 0; i < 2 * CH; i++) {
+                const float4 u = *reinterpret_cast<const float4*>(qp + 32 * (i >> 1) + 4 * (i & 1));
+                most = fmaxf(fmaxf(most, fmaxf(fabsf(u.x), fabsf(u.y))), fmaxf(fabsf(u.z), fabsf(u.w)));
             }
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
             // the head's largest |q| comes to [1, 2); 2^-126 and less count as 2^-126 (the floor of E covers them)
             const int e = max(-126, min(127, (int)(__float_as_uint(most) >> 23) - 127));
             const float down0 = pow2(-(e / 2)), down1 = pow2(-(e - e / 2));  // 2^-e in two factors, each of them normal
-            int e_max = gid < G && most > 0.f ? e : -126;
+            int e_max = e;
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) e_max = max(e_max, __shfl_xor_sync(0xffffffffu, e_max, o));
-            const float f = gid < G ? pow2(max(-126, e - e_max)) : 0.f;
+            const float f = pow2(max(-126, e - e_max));
             f0 = __shfl_sync(0xffffffffu, f, 8 * tig);
             f1 = __shfl_sync(0xffffffffu, f, 8 * tig + 4);
             auto split = [](float a, float b, unsigned& hi, unsigned& lo) {
@@ -235,7 +238,9 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
                 const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&hi));
                 lo = half2_bits((a - t.x) * 2048.f, (b - t.y) * 2048.f);
             };
-            if (warp < CH) {
+            if (warp < CH) {  // each warp lays out one chunk of the dims; word j of a part: dims 2j, 2j + 1 of the lane's eight
+                const float4 u = *reinterpret_cast<const float4*>(qp + 32 * warp), v = *reinterpret_cast<const float4*>(qp + 32 * warp + 4);
+                const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
                 unsigned w[4][4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -249,29 +254,26 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
             }
         }
         __syncthreads();
-        float err = 0.f, mn = INFINITY, mx = -INFINITY;
+        // E is never negative, so its bits order as it does, and an infinity or a NaN (0 * inf) is above every number
+        unsigned err_bits = 0;
+        float mn = INFINITY, mx = -INFINITY;
+        const float k0 = 0x1p-13f * f0, k1 = 0x1p-13f * f1, floor0 = 0x1p-12f * f0, floor1 = 0x1p-12f * f1;
+        const uint8_t* bounds = static_cast<const uint8_t*>(c.key_bounds) + (size_t)kvh * 4 * HD + 16 * tig;
+        const size_t block_bytes = (size_t)c.n_kv_heads * 4 * HD;
         for (; b0 < own; b0 += kSelRun) {
             const bool ok0 = paged_block_ok(page0, c.n_blocks), ok1 = paged_block_ok(page1, c.n_blocks);
-            const size_t head = (size_t)c.n_kv_heads, bytes = 4 * HD;
-            const uint8_t* p0 = static_cast<const uint8_t*>(c.key_bounds) + ((size_t)(ok0 ? page0 : 0) * head + kvh) * bytes + 16 * tig;
-            const uint8_t* p1 = static_cast<const uint8_t*>(c.key_bounds) + ((size_t)(ok1 ? page1 : 0) * head + kvh) * bytes + 16 * tig;
+            // (what is not mapped is read from the null block and does not count)
+            const uint8_t *p0 = bounds + (ok0 ? page0 : 0) * block_bytes, *p1 = bounds + (ok1 ? page1 : 0) * block_bytes;
             uint4 l0[CH], l1[CH], h0[CH], h1[CH];
 #pragma unroll
             for (int i = 0; i < CH; i++) {
-                const uint4 z = make_uint4(0, 0, 0, 0);
-                l0[i] = ok0 ? __ldg(reinterpret_cast<const uint4*>(p0 + 64 * i)) : z;
-                h0[i] = ok0 ? __ldg(reinterpret_cast<const uint4*>(p0 + 2 * HD + 64 * i)) : z;
-                l1[i] = ok1 ? __ldg(reinterpret_cast<const uint4*>(p1 + 64 * i)) : z;
-                h1[i] = ok1 ? __ldg(reinterpret_cast<const uint4*>(p1 + 2 * HD + 64 * i)) : z;
+                h0[i] = load16(p0 + 2 * HD + 64 * i);
+                h1[i] = load16(p1 + 2 * HD + 64 * i);
+                l0[i] = load16(p0 + 64 * i);
+                l1[i] = load16(p1 + 64 * i);
             }
-            // the next run's bounds are on their way to L2 (a line a lane), the one's after it pages to registers
-            const size_t line = (size_t)128 * tig;
-            if (line < bytes && paged_block_ok(next0, c.n_blocks)) prefetch_l2(static_cast<const uint8_t*>(c.key_bounds) + ((size_t)next0 * head + kvh) * bytes + line);
-            if (line < bytes && paged_block_ok(next1, c.n_blocks)) prefetch_l2(static_cast<const uint8_t*>(c.key_bounds) + ((size_t)next1 * head + kvh) * bytes + line);
-            page0 = next0;
-            page1 = next1;
-            next0 = page_of(b0 + 2 * kSelRun + gid);
-            next1 = page_of(b0 + 2 * kSelRun + 8 + gid);
+            page0 = page_of(b0 + kSelRun + gid);
+            page1 = page_of(b0 + kSelRun + 8 + gid);
             float hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0}, up[4] = {0, 0, 0, 0}, dn[4] = {0, 0, 0, 0};
             constexpr unsigned abs2 = 0x7fff7fffu;
             // two k steps on a chunk of the bounds: words 0, 1 and words 2, 3
@@ -289,41 +291,29 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const b200_pa
                 chunk(l0[i], l1[i], q_frag[i][2][lane], q_frag[i][3][lane], dn);
             }
             // columns 2 tig and 2 tig + 1 of rows gid (values 0, 1) and gid + 8 (values 2, 3)
-            float s[2], E[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const float S0 = up[2 * h] - dn[2 * h], S1 = up[2 * h + 1] - dn[2 * h + 1];
-                const float s0 = fmaf(lo[2 * h], 0x1p-11f, hi[2 * h]) * f0, s1 = fmaf(lo[2 * h + 1], 0x1p-11f, hi[2 * h + 1]) * f1;
-                const float E0 = fmaf(S0, 0x1p-13f, 0x1p-12f) * f0, E1 = fmaf(S1, 0x1p-13f, 0x1p-12f) * f1;
-                const bool in0 = 2 * tig < G, in1 = 2 * tig + 1 < G;
-                s[h] = fmaxf(in0 ? s0 : -INFINITY, in1 ? s1 : -INFINITY);
-                E[h] = fmaxf(in0 ? E0 : 0.f, in1 ? E1 : 0.f);
-                // an infinity or a NaN shows in S (0 * inf) or in s
-                if ((in0 && !(fabsf(E0) + fabsf(s0) < 3e38f)) || (in1 && !(fabsf(E1) + fabsf(s1) < 3e38f))) E[h] = INFINITY;
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) {
-                    s[h] = fmaxf(s[h], __shfl_xor_sync(0xffffffffu, s[h], o));
-                    E[h] = fmaxf(E[h], __shfl_xor_sync(0xffffffffu, E[h], o));
-                }
-            }
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const bool ok = h ? ok1 : ok0;
                 const int b = b0 + 8 * h + gid;
+                const float E0 = fmaf(up[2 * h] - dn[2 * h], k0, floor0), E1 = fmaf(up[2 * h + 1] - dn[2 * h + 1], k1, floor1);
+                float s = fmaxf(fmaf(lo[2 * h], 0x1p-11f, hi[2 * h]) * f0, fmaf(lo[2 * h + 1], 0x1p-11f, hi[2 * h + 1]) * f1);
+                s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 1));
+                s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 2));
                 if (ok) {
-                    err = fmaxf(err, E[h]);
-                    mn = fminf(mn, s[h]);
-                    mx = fmaxf(mx, s[h]);
+                    err_bits = max(err_bits, max(__float_as_uint(E0) & 0x7fffffffu, __float_as_uint(E1) & 0x7fffffffu));
+                    mn = fminf(mn, s);
+                    mx = fmaxf(mx, s);
                 }
-                if (tig == 0 && b < own) sel_score[b] = ok ? s[h] : -INFINITY;
+                if (tig == 0 && b < own) sel_score[b] = ok ? s : -INFINITY;
             }
         }
+        err_bits = __reduce_max_sync(0xffffffffu, err_bits);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
-            err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, o));
             mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         }
+        const float err = __uint_as_float(min(err_bits, 0x7f800000u));
         if (ctas > 1) cluster_wait();  // the CTAs have started: their shared memory may be written
         const int at = rank * kSelWarps + warp;
         tell(s_err + at, err);
