@@ -171,10 +171,16 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
 }
 
 // ---- append ----------------------------------------------------------------------------------------------------------
-// Packed rows whose slots follow one another inside one block are a run; the first row of a run stores the whole run, so a
-// block's bounds are written once and see every key: lo_d = min, hi_d = max over the block's rows 0 .. last of the fp16
-// keys, the older ones read back from the pool. NaN keys make NaN bounds (min.NaN / max.NaN). A warp takes (run, kv head),
-// a lane HD/32 dims. Bytes bound it: 8 HD in and 4 HD out a row and head.
+// Packed rows whose slots follow one another inside one block are a run; the CTA that holds a run's first row stores the whole
+// run, so a block's bounds are written once and see every key: lo_d = min, hi_d = max over the block's rows 0 .. last of the
+// fp16 keys, the older ones read back from the pool. NaN keys make NaN bounds (min.NaN / max.NaN).
+//
+// Bytes bound it: 8 HD in and 4 HD out a row and head. A warp takes a kv head of the run (four dims a lane, one row of 128 or two
+// of 64 at a time) with four loads of k and of v in flight (with eight, at twice the
+// registers, 8192-row prompts run alike and decode rows 0.2 us slower); where there are fewer heads than warps, several warps share a
+// head's rows and join their bounds in shared memory.
+constexpr int kAppendMaxWarps = 16;
+
 __device__ __forceinline__ unsigned min_nan2(unsigned a, unsigned b) {
     unsigned r;
     asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -185,65 +191,101 @@ __device__ __forceinline__ unsigned max_nan2(unsigned a, unsigned b) {
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-
-template <int HD>
-struct LaneRow;  // a lane's share of a row: HD/32 floats in, as many halves out
-template <>
-struct LaneRow<128> {
-    using In = float4;
-    using Out = uint2;
-    static __device__ __forceinline__ Out pack(In x) {
-        const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
-        return make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
-    }
-    static __device__ __forceinline__ void fold(Out& lo, Out& hi, Out x) {
-        lo.x = min_nan2(lo.x, x.x); lo.y = min_nan2(lo.y, x.y);
-        hi.x = max_nan2(hi.x, x.x); hi.y = max_nan2(hi.y, x.y);
+struct Bounds4 {  // of four dims
+    uint2 lo = {0x7c007c00u, 0x7c007c00u}, hi = {0xfc00fc00u, 0xfc00fc00u};  // +inf, -inf
+    __device__ __forceinline__ void fold(uint2 l, uint2 h) {
+        lo.x = min_nan2(lo.x, l.x); lo.y = min_nan2(lo.y, l.y);
+        hi.x = max_nan2(hi.x, h.x); hi.y = max_nan2(hi.y, h.y);
     }
 };
-template <>
-struct LaneRow<64> {
-    using In = float2;
-    using Out = unsigned;
-    static __device__ __forceinline__ Out pack(In x) {
-        const __half2 a = __floats2half2_rn(x.x, x.y);
-        return *reinterpret_cast<const unsigned*>(&a);
-    }
-    static __device__ __forceinline__ void fold(Out& lo, Out& hi, Out x) { lo = min_nan2(lo, x); hi = max_nan2(hi, x); }
-};
+__device__ __forceinline__ uint2 to_half4(float4 x) {
+    const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+    return make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+}
 
+// rows_per_cta: packed rows whose runs a CTA looks for; parts: warps that share a head (when above 1, the CTA has heads * parts warps)
 template <int HD>
-__global__ void __launch_bounds__(256) paged_append_kernel(const b200_paged_cache c, const int32_t* __restrict__ slot_map, int n_rows,
-                                                           const float* __restrict__ k, size_t ldk, const float* __restrict__ v, size_t ldv) {
-    using L = LaneRow<HD>;
-    using In = typename L::In;
-    using Out = typename L::Out;
-    const int r = blockIdx.x, lane = threadIdx.x & 31, br = c.block_rows;
-    const int at = slot_map[r];
-    if (at < 0 || !paged_block_ok(at / br, c.n_blocks)) return;
-    const int block = at / br, first = at % br;
-    if (first > 0 && r > 0 && slot_map[r - 1] == at - 1) return;  // an earlier row of the run stores this one
-    int n = 1;
-    while (first + n < br && r + n < n_rows && slot_map[r + n] == at + n) n++;
-    for (int h = threadIdx.x >> 5; h < c.n_kv_heads; h += blockDim.x >> 5) {
-        const size_t tile = paged_tile(block, h, c.n_kv_heads, br, HD);
-        Out* kt = reinterpret_cast<Out*>(static_cast<__half*>(c.k_pool) + tile) + lane;
-        Out* vt = reinterpret_cast<Out*>(static_cast<__half*>(c.v_pool) + tile) + lane;
-        constexpr int RS = 32;  // Out elements between rows of a tile
-        Out lo, hi;
-        for (int j = 0; j < n; j++) {
-            const Out ko = L::pack(reinterpret_cast<const In*>(k + (size_t)(r + j) * ldk + (size_t)h * HD)[lane]);
-            const Out vo = L::pack(reinterpret_cast<const In*>(v + (size_t)(r + j) * ldv + (size_t)h * HD)[lane]);
-            kt[(first + j) * RS] = ko;
-            vt[(first + j) * RS] = vo;
-            if (j == 0) { lo = ko; hi = ko; }
-            else L::fold(lo, hi, ko);
+__global__ void __launch_bounds__(32 * kAppendMaxWarps) paged_append_kernel(const b200_paged_cache c, const int32_t* __restrict__ slot_map, int n_rows,
+                                                                            const float* __restrict__ k, size_t ldk, const float* __restrict__ v,
+                                                                            size_t ldv, int rows_per_cta, int parts) {
+    constexpr int LPR = HD / 4, RPW = 32 / LPR, U = 4;  // lanes a row, rows a warp at a time, loads in flight
+    __shared__ Bounds4 joined[kAppendMaxWarps][LPR];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, br = c.block_rows;
+    const int sub = lane % LPR, row_of = lane / LPR;
+    // the first rows of runs among this CTA's rows, a lane a row
+    const int mine = blockIdx.x * rows_per_cta + lane;
+    bool starts = false;
+    if (lane < rows_per_cta && mine < n_rows) {
+        const int at = slot_map[mine], before = mine > 0 ? slot_map[mine - 1] : -1;
+        starts = at >= 0 && paged_block_ok(at / br, c.n_blocks) && (before != at - 1 || at % br == 0);
+    }
+    for (unsigned todo = __ballot_sync(0xffffffffu, starts); todo; todo &= todo - 1u) {
+        const int r = blockIdx.x * rows_per_cta + __ffs((int)todo) - 1, at = slot_map[r], block = at / br, first = at % br;
+        const int most = min(br - first, n_rows - r);
+        int n = 0;
+        while (n < most) {
+            const unsigned here = __ballot_sync(0xffffffffu, n + lane < most && slot_map[r + n + lane] == at + n + lane);
+            n += here == 0xffffffffu ? 32 : __ffs((int)~here) - 1;
+            if (here != 0xffffffffu) break;
         }
-        if (!c.key_bounds) continue;
-        for (int j = 0; j < first; j++) L::fold(lo, hi, kt[j * RS]);
-        Out* b = reinterpret_cast<Out*>(static_cast<__half*>(c.key_bounds) + ((size_t)block * c.n_kv_heads + h) * 2 * HD) + lane;
-        b[0] = lo;
-        b[RS] = hi;
+        for (int u = warp; u < c.n_kv_heads * parts; u += warps) {
+            const int h = u % c.n_kv_heads, part = u / c.n_kv_heads;
+            const size_t tile = paged_tile(block, h, c.n_kv_heads, br, HD);
+            uint2* kt = reinterpret_cast<uint2*>(static_cast<__half*>(c.k_pool) + tile) + sub;
+            uint2* vt = reinterpret_cast<uint2*>(static_cast<__half*>(c.v_pool) + tile) + sub;
+            const float4* ks = reinterpret_cast<const float4*>(k + (size_t)r * ldk + (size_t)h * HD) + sub;
+            const float4* vs = reinterpret_cast<const float4*>(v + (size_t)r * ldv + (size_t)h * HD) + sub;
+            Bounds4 bounds;
+            const int j0 = n * part / parts, j1 = n * (part + 1) / parts;
+            for (int j = j0 + row_of; j < j1; j += U * RPW) {
+                float4 kx[U], vx[U];
+#pragma unroll
+                for (int i = 0; i < U; i++) {
+                    if (j + i * RPW < j1) {
+                        kx[i] = __ldcs(ks + (size_t)(j + i * RPW) * (ldk / 4));
+                        vx[i] = __ldcs(vs + (size_t)(j + i * RPW) * (ldv / 4));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < U; i++) {
+                    if (j + i * RPW < j1) {
+                        const uint2 ko = to_half4(kx[i]);
+                        const size_t to = (size_t)(first + j + i * RPW) * LPR;
+                        kt[to] = ko;
+                        vt[to] = to_half4(vx[i]);
+                        bounds.fold(ko, ko);
+                    }
+                }
+            }
+            if (!c.key_bounds) continue;
+            const int o0 = first * part / parts, o1 = first * (part + 1) / parts;
+            for (int j = o0 + row_of; j < o1; j += U * RPW) {
+                uint2 old[U];
+#pragma unroll
+                for (int i = 0; i < U; i++)
+                    if (j + i * RPW < o1) old[i] = kt[(size_t)(j + i * RPW) * LPR];
+#pragma unroll
+                for (int i = 0; i < U; i++)
+                    if (j + i * RPW < o1) bounds.fold(old[i], old[i]);
+            }
+            if constexpr (RPW == 2) {
+                const uint2 l = make_uint2(__shfl_xor_sync(0xffffffffu, bounds.lo.x, 16), __shfl_xor_sync(0xffffffffu, bounds.lo.y, 16));
+                const uint2 g = make_uint2(__shfl_xor_sync(0xffffffffu, bounds.hi.x, 16), __shfl_xor_sync(0xffffffffu, bounds.hi.y, 16));
+                bounds.fold(l, g);
+            }
+            if (parts > 1) {
+                if (row_of == 0) joined[warp][sub] = bounds;
+                __syncthreads();
+                if (part == 0)
+                    for (int p = 1; p < parts; p++) bounds.fold(joined[warp + p * c.n_kv_heads][sub].lo, joined[warp + p * c.n_kv_heads][sub].hi);
+                __syncthreads();
+            }
+            if (part == 0 && row_of == 0) {
+                uint2* b = reinterpret_cast<uint2*>(static_cast<__half*>(c.key_bounds) + ((size_t)block * c.n_kv_heads + h) * 2 * HD) + sub;
+                b[0] = bounds.lo;
+                b[LPR] = bounds.hi;
+            }
+        }
     }
 }
 
@@ -316,11 +358,16 @@ extern "C" int b200_paged_append(b200_ctx* ctx, const b200_paged_cache* c, const
     if (ctx->device < 0) B200_FAIL(ctx, B200_CUDA_ERROR, "b200_paged_append: the context has no device");
     DeviceScope dev;
     CUDA_TRY(ctx, dev.enter(ctx->device));
-    const int warps = c->n_kv_heads < 8 ? c->n_kv_heads : 8;
-    if (c->head_dim == 128)
-        paged_append_kernel<128><<<r->n_rows, warps * 32, 0, ctx->stream>>>(*c, r->slot_map, r->n_rows, k, (size_t)ldk, v, (size_t)ldv);
-    else
-        paged_append_kernel<64><<<r->n_rows, warps * 32, 0, ctx->stream>>>(*c, r->slot_map, r->n_rows, k, (size_t)ldk, v, (size_t)ldv);
+    // Few rows are decode steps: a CTA looks at one, and with tall blocks sixteen warps share the older rows to be read. Many rows
+    // are prompts, whose runs fill blocks: a CTA that finds no run among its rows costs about as much as 4 ns of the GPU, so it
+    // looks at more (32768 rows of 8 heads of 128 in blocks of 64: 139, 82, 74, 68 us with 1, 4, 8, 32 rows a CTA; 2115 rows in
+    // seven chunks with blocks of 32: 8.1, 5.3, 5.5, 7.2 us).
+    const int rows = r->n_rows > 32 * ctx->sm_count ? 32 : r->n_rows > 4 * ctx->sm_count ? 4 : 1;
+    const int warps = rows > 1 || c->block_rows < 32 ? 8 : kAppendMaxWarps;
+    const int parts = c->n_kv_heads < warps ? warps / c->n_kv_heads : 1;
+    const int threads = 32 * (c->n_kv_heads < warps ? c->n_kv_heads * parts : warps);
+    auto kernel = c->head_dim == 128 ? paged_append_kernel<128> : paged_append_kernel<64>;
+    kernel<<<ceil_div(r->n_rows, rows), threads, 0, ctx->stream>>>(*c, r->slot_map, r->n_rows, k, (size_t)ldk, v, (size_t)ldv, rows, parts);
     LAUNCH_CHECK(ctx);
     return B200_OK;
 }
