@@ -29,27 +29,45 @@ def _refuse(text: str):
     raise ResidentError(abi.BAD_ARGUMENT, text)
 
 
-_NAMES: dict = {}  # dtype -> its text (formatting one costs more than a whole check)
+_F32, _F16, _I32 = "torch.float32", "torch.float16", "torch.int32"
+_names: dict = {}  # dtype -> its text: formatting one costs more than a whole check
 
 
 def _is(dtype, name: str) -> bool:
-    text = _NAMES.get(dtype)
+    text = _names.get(dtype)
     if text is None:
-        text = _NAMES[dtype] = str(dtype)
+        text = _names[dtype] = str(dtype)
     return text == name
 
 
-def _array(name: str, a, dtype: str, shape, device: int):
+def _array(name: str, a, dtype: str, shape, device: int) -> int:
     """Address of a contiguous device array of this type and shape (None entries of shape: any extent)."""
+    if a.shape == shape and _names.get(a.dtype) == dtype and a.get_device() == device and a.is_contiguous():
+        return a.data_ptr()
     if not _is(a.dtype, dtype):
         _refuse(f"{name} has type {a.dtype}, not {dtype}")
-    if a.shape != shape and (len(a.shape) != len(shape) or any(w is not None and n != w for n, w in zip(a.shape, shape))):
+    if len(a.shape) != len(shape) or any(w is not None and n != w for n, w in zip(a.shape, shape)):
         _refuse(f"{name} has shape {tuple(a.shape)}, not {tuple('any' if w is None else w for w in shape)}")
     if a.get_device() != device:
         _refuse(f"{name} is on {a.device}, the context on cuda:{device}")
     if not a.is_contiguous():
         _refuse(f"{name} is not contiguous")
     return a.data_ptr()
+
+
+def _packed(name: str, a, n_rows: int, device: int):
+    """Address, row stride and row width of a f32 [n_rows][...] device array whose rows are contiguous."""
+    shape, stride = a.shape, a.stride()
+    if len(shape) == 2 and stride[1] == 1 and shape[0] == n_rows and _names.get(a.dtype) == _F32 and a.get_device() == device:
+        return a.data_ptr(), stride[0] if n_rows > 1 else shape[1], shape[1]
+    if len(shape) < 2 or shape[0] != n_rows or not _is(a.dtype, _F32) or a.get_device() != device:
+        _refuse(f"{name} is {a.dtype} {tuple(shape)} on {a.device}, not f32 with {n_rows} rows on cuda:{device}")
+    width = 1
+    for n, st in zip(shape[:0:-1], stride[:0:-1]):
+        if n != 1 and st != width:
+            _refuse(f"the rows of {name} are not contiguous (shape {tuple(shape)}, strides {stride})")
+        width *= n
+    return a.data_ptr(), stride[0] if n_rows > 1 else width, width
 
 
 class PagedRows:
@@ -64,12 +82,12 @@ class PagedRows:
         self.n_seqs = None if seq_row0 is None else seq_row0.shape[0] - 1
         self._keep = (row_slot, row_pos, slot_map, seq_row0, status)
         self.row_slot, self.row_pos, self.slot_map, self.seq_row0, self.status = self._keep
-        i32 = "torch.int32"
+        i32 = _I32
         self.c = abi.PagedRows(None if seq_row0 is None else _array("seq_row0", seq_row0, i32, (None,), device),
                                _array("row_slot", row_slot, i32, (n,), device), _array("row_pos", row_pos, i32, (n,), device),
                                None if slot_map is None else _array("slot_map", slot_map, i32, (n,), device),
                                None if status is None else _array("status", status, i32, (4,), device), n, 0)
-        self.ref = C.byref(self.c)
+        self._c = C.addressof(self.c)
 
 
 class PagedCache:
@@ -79,7 +97,7 @@ class PagedCache:
 
     def __init__(self, ops, block_table, seq_blocks, free_blocks, free_count, block_rows: int, k_pool=None, v_pool=None, key_bounds=None):
         self.ops, self.device = ops, ops.drv.device
-        dev, i32, f16 = self.device, "torch.int32", "torch.float16"
+        dev, i32, f16 = self.device, _I32, _F16
         self._keep = (block_table, seq_blocks, free_blocks, free_count, k_pool, v_pool, key_bounds)
         table = _array("block_table", block_table, i32, (None, None), dev)
         self.n_seqs, max_blocks = block_table.shape
@@ -101,7 +119,7 @@ class PagedCache:
                                 None if key_bounds is None else _array("key_bounds", key_bounds, f16, (n_blocks, kv, 2, hd), dev), table,
                                 _array("seq_blocks", seq_blocks, i32, (self.n_seqs,), dev), _array("free_blocks", free_blocks, i32, (n_blocks,), dev),
                                 _array("free_count", free_count, i32, (1,), dev), n_blocks, self.n_seqs, max_blocks, block_rows, kv, hd)
-        self.ref = C.byref(self.c)
+        self._c, self._ctx = C.addressof(self.c), ops.ctx.value
         lib = ops.lib
         vp, i, f = C.c_void_p, C.c_int, C.c_float
         for fn, types in ((lib.b200_paged_plan, (vp, vp, vp, vp, vp)), (lib.b200_paged_append, (vp, vp, vp, vp, i, vp, i)),
@@ -113,24 +131,10 @@ class PagedCache:
     def _raise(self, st: int):
         raise ResidentError(st, self.ops.drv.last_error())
 
-    def _packed(self, name: str, a, rows: PagedRows):
-        """Address, row stride and row width of a f32 [n_rows][...] device array whose rows are contiguous."""
-        shape, stride, n_rows = a.shape, a.stride(), rows.n_rows
-        if len(shape) == 2 and stride[1] == 1:
-            width = shape[1]
-        else:
-            width = 1
-            for n, st in zip(shape[:0:-1], stride[:0:-1]):
-                if n != 1 and st != width:
-                    _refuse(f"the rows of {name} are not contiguous (shape {tuple(shape)}, strides {stride})")
-                width *= n
-        if shape[0] != n_rows or not _is(a.dtype, "torch.float32") or a.get_device() != self.device or rows.device != self.device:
-            _refuse(f"{name} is {a.dtype} {tuple(shape)} on {a.device}, not f32 with {n_rows} rows on cuda:{self.device}, or the rows are not there")
-        return a.data_ptr(), stride[0] if n_rows > 1 else width, width
-
-    def _lists(self, sel, rows: PagedRows):
-        shape = sel.shape
-        return _array("sel", sel, "torch.int32", (rows.n_rows, self.n_kv_heads, shape[-1]), self.device), shape[-1]
+    def _here(self, rows: PagedRows) -> int:
+        if rows.device != self.device:
+            _refuse(f"the rows are on cuda:{rows.device}, the cache is on cuda:{self.device}")
+        return rows.n_rows
 
     def _heads(self, name: str, width: int) -> int:
         if self.head_dim == 0 or width % self.head_dim:
@@ -138,35 +142,41 @@ class PagedCache:
         return width // self.head_dim
 
     def plan(self, kv_len, n_new, rows: PagedRows):
-        if rows.n_seqs != self.n_seqs or rows.device != self.device:
-            _refuse(f"rows are for {rows.n_seqs} sequences on cuda:{rows.device}, the cache has {self.n_seqs} on cuda:{self.device}")
-        st = self._plan(self.ops.ctx, self.ref, rows.ref, _array("kv_len", kv_len, "torch.int32", (self.n_seqs,), self.device),
-                        _array("n_new", n_new, "torch.int32", (self.n_seqs,), self.device))
+        self._here(rows)
+        if rows.n_seqs != self.n_seqs:
+            _refuse(f"rows are for {rows.n_seqs} sequences, the cache has {self.n_seqs}")
+        shape, device = (self.n_seqs,), self.device
+        st = self._plan(self._ctx, self._c, rows._c, _array("kv_len", kv_len, _I32, shape, device), _array("n_new", n_new, _I32, shape, device))
         if st:
             self._raise(st)
 
     def append(self, rows: PagedRows, k, v):
-        pk, ldk, wk = self._packed("k", k, rows)
-        pv, ldv, wv = self._packed("v", v, rows)
+        n, device = self._here(rows), self.device
+        pk, ldk, wk = _packed("k", k, n, device)
+        pv, ldv, wv = _packed("v", v, n, device)
         if wk != self.n_kv_heads * self.head_dim or wv != wk:
             _refuse(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have {self.n_kv_heads} heads of {self.head_dim} a row")
-        st = self._append(self.ops.ctx, self.ref, rows.ref, pk, ldk, pv, ldv)
+        st = self._append(self._ctx, self._c, rows._c, pk, ldk, pv, ldv)
         if st:
             self._raise(st)
 
     def select(self, rows: PagedRows, q, sel, n_first: int = 1, n_recent: int = 1):
-        p, n = self._lists(sel, rows)
-        pq, ldq, width = self._packed("q", q, rows)
-        st = self._select(self.ops.ctx, self.ref, rows.ref, pq, ldq, self._heads("q", width), n_first, n_recent, n, p)
+        n, device = self._here(rows), self.device
+        pq, ldq, width = _packed("q", q, n, device)
+        n_select = sel.shape[-1]
+        ps = _array("sel", sel, _I32, (n, self.n_kv_heads, n_select), device)
+        st = self._select(self._ctx, self._c, rows._c, pq, ldq, self._heads("q", width), n_first, n_recent, n_select, ps)
         if st:
             self._raise(st)
 
     def attend(self, rows: PagedRows, q, sel, out, scale: float = 0.0, softcap: float = 0.0):
-        p, n = self._lists(sel, rows)
-        pq, ldq, width = self._packed("q", q, rows)
-        po, ldo, wide = self._packed("out", out, rows)
+        n, device = self._here(rows), self.device
+        pq, ldq, width = _packed("q", q, n, device)
+        po, ldo, wide = _packed("out", out, n, device)
         if wide != width:
             _refuse(f"out has shape {tuple(out.shape)}, q {tuple(q.shape)}")
-        st = self._attend(self.ops.ctx, self.ref, rows.ref, pq, ldq, self._heads("q", width), scale, softcap, p, n, po, ldo)
+        n_select = sel.shape[-1]
+        ps = _array("sel", sel, _I32, (n, self.n_kv_heads, n_select), device)
+        st = self._attend(self._ctx, self._c, rows._c, pq, ldq, self._heads("q", width), scale, softcap, ps, n_select, po, ldo)
         if st:
             self._raise(st)
