@@ -8,8 +8,9 @@
 // pushed as number S-1-e, and element k of the new blocks is popped as number k: what the k-th new block pops is
 // stack[count + S - 1 - k], which for k < S is the k-th released block. Three scans (rows, grow, shrink) over the sequences
 // place everything; each released block, new block and row then finds its sequence by a search in the scan.
-// The kernel is latency: one launch of one cluster, whose CTAs each make the scans for themselves (a few ints a sequence)
-// and share the elements out. Cluster barriers stand between the reads of the old state, the pushes and the pops.
+// The scans are latency (a chain of loads, a scan, loads), so one CTA makes them; with many blocks to move it is a cluster, whose
+// CTAs each make the scans for themselves and share the blocks out. Barriers stand between the reads of the old state, the
+// pushes and the pops. Up to 2048 rows are written by the same launch, more by a second kernel over the whole GPU.
 #include "paged.cuh"
 
 namespace {
@@ -26,16 +27,25 @@ struct PlanArgs {
     const int32_t* n_new;
     int32_t *row0, *row_slot, *row_pos, *slot_map, *status;
     int n_seqs, n_blocks, max_blocks, block_rows, n_rows;
+    unsigned by_rows;  // division by block_rows: paged_divisor
+    int top_step;      // the first step of a search among n_seqs
 };
 
 // the last index i with scan[i] <= e, for e < scan[n] (empty sequences are stepped over)
-__device__ __forceinline__ int find_owner(const int* scan, int n, int e) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (scan[mid] <= e) lo = mid; else hi = mid;
-    }
-    return lo;
+__device__ __forceinline__ int find_owner(const int* scan, int n, int top_step, int e) {
+    int at = 0;
+    for (int step = top_step; step > 0; step >>= 1)
+        if (at + step < n && scan[at + step] <= e) at += step;
+    return at;
+}
+
+// the packed row r, whose sequence is i and starts at row `first`
+__device__ __forceinline__ void write_row(const PlanArgs& a, int r, int i, int first, int len) {
+    const int pos = len + r - first, p = (int)paged_div((unsigned)pos, a.by_rows);
+    const int block = __ldcg(a.table + (size_t)i * a.max_blocks + p);
+    a.row_slot[r] = i;
+    a.row_pos[r] = pos;
+    a.slot_map[r] = paged_block_ok(block, a.n_blocks) ? block * a.block_rows + (pos - p * a.block_rows) : -1;
 }
 
 struct Sums {
@@ -53,7 +63,8 @@ __device__ __forceinline__ Sums warp_inclusive(Sums v, int lane) {
     return v;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs a) {
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs a, int write_rows) {
+    pdl_trigger();  // the rows' kernel waits for this one's end
     extern __shared__ int plan_smem[];
     int* row0 = plan_smem;                    // [n + 1] scan of new rows
     int* grow0 = row0 + a.n_seqs + 1;         // [n + 1] scan of blocks taken
@@ -64,21 +75,24 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
     if (tid == 0) first_bad = n;
     __syncthreads();
 
-    // every thread takes a run of sequences; two reads of the lengths, the second from the cache
+    // every thread takes a run of sequences; with more than one it looks at them again for the scan
     const int per = (n + kPlanThreads - 1) / kPlanThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
-    auto look = [&](int i, int& want, int& have) {
-        const int len = a.kv_len[i], add = a.n_new[i];
+    const int free0 = *a.count;
+    int add = 0, want = 0, have = 0;
+    auto look = [&](int i) {
+        const int len = a.kv_len[i];
+        add = a.n_new[i];
         have = a.seq_blocks[i];
         const long long all = (long long)len + add;
         const bool bad = len < 0 || add < 0 || all > (long long)a.max_blocks * br || have < 0 || have > a.max_blocks || len > (long long)have * br;
-        want = bad ? have : (int)((all + br - 1) / br);
-        return !bad;
+        if (bad) atomicMin(&first_bad, i);
+        want = bad ? have : (int)paged_div_up((unsigned)all, a.by_rows);
+        if (bad) add = 0;
     };
     Sums mine{0, 0, 0};
     for (int i = i0; i < i1; i++) {
-        int want, have;
-        if (!look(i, want, have)) { atomicMin(&first_bad, i); continue; }
-        mine.rows += a.n_new[i];
+        look(i);
+        mine.rows += add;
         mine.grow += max(0, want - have);
         mine.shrink += max(0, have - want);
     }
@@ -100,73 +114,86 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
         scan.shrink += warp_sum[warp - 1].shrink;
     }
     for (int i = i0; i < i1; i++) {
-        int want, have;
-        const bool good = look(i, want, have);
+        if (per > 1) look(i);
         row0[i] = (int)scan.rows;  // used only when the rows fit n_rows
         grow0[i] = scan.grow;
         shrink0[i] = scan.shrink;
-        if (good) {
-            scan.rows += a.n_new[i];
-            scan.grow += max(0, want - have);
-            scan.shrink += max(0, have - want);
-        }
+        scan.rows += add;
+        scan.grow += max(0, want - have);
+        scan.shrink += max(0, have - want);
     }
+    const int G = total.grow, S = total.shrink;
     if (tid == 0) {
         row0[n] = (int)total.rows;
-        grow0[n] = total.grow;
-        shrink0[n] = total.shrink;
+        grow0[n] = G;
+        shrink0[n] = S;
     }
-    const int free0 = *a.count, G = total.grow, S = total.shrink;
     const int bad_seq = first_bad;
     const bool bad = bad_seq < n || total.rows > a.n_rows || free0 < 0 || (long long)free0 + S > a.n_blocks;
     const bool full = !bad && G > free0 + S;
     const int rank = (int)cluster_rank(), ctas = (int)cluster_size();
     const int gtid = rank * kPlanThreads + tid, step = ctas * kPlanThreads;
-    cluster_sync();  // the old state has been read by every CTA
+    auto everyone = [&] {
+        if (ctas > 1) cluster_sync(); else __syncthreads();
+    };
+    everyone();  // the old state has been read by every CTA
 
-    if (rank == 0 && tid == 0) {
+    if (gtid == 0) {
         a.status[0] = bad ? B200_BAD_ARGUMENT : full ? B200_KV_POOL_FULL : B200_OK;
         a.status[1] = bad || full ? 0 : (int)total.rows;
         a.status[2] = bad || full ? free0 : free0 + S - G;
         a.status[3] = bad ? bad_seq : full ? G - free0 - S : 0;
         if (!bad && !full) *a.count = free0 + S - G;
     }
-    if (bad || full) {  // nothing changes, and no row takes part in what follows
-        for (int r = gtid; r < a.n_rows; r += step) a.row_slot[r] = a.row_pos[r] = a.slot_map[r] = -1;
-        for (int i = gtid; i <= n; i += step) a.row0[i] = 0;
-        return;
-    }
-    auto want_of = [&](int i) { return (int)(((unsigned)a.kv_len[i] + (unsigned)a.n_new[i] + (unsigned)br - 1u) / (unsigned)br); };
-    for (int e = gtid; e < S; e += step) {
-        const int i = find_owner(shrink0, n, e);
-        int32_t* entry = a.table + (size_t)i * a.max_blocks + want_of(i) + (e - shrink0[i]);
-        a.stack[free0 + S - 1 - e] = *entry;
-        *entry = 0;
-    }
-    if (rank == 0)
-        for (int i = tid; i < n; i += kPlanThreads) a.seq_blocks[i] = want_of(i);
-    for (int i = gtid; i <= n; i += step) a.row0[i] = row0[i];
-    cluster_sync();  // the pushes are on the stack
-
-    for (int k = gtid; k < G; k += step) {
-        const int i = find_owner(grow0, n, k);
-        const int have = want_of(i) - (grow0[i + 1] - grow0[i]);
-        a.table[(size_t)i * a.max_blocks + have + (k - grow0[i])] = __ldcg(a.stack + free0 + S - 1 - k);
-    }
-    for (int r = gtid; r < a.n_rows; r += step) {
-        int slot = -1, pos = -1, at = -1;
-        if (r < (int)total.rows) {
-            slot = find_owner(row0, n, r);
-            pos = a.kv_len[slot] + r - row0[slot];
-            const int p = pos / br, grown = grow0[slot + 1] - grow0[slot], have = want_of(slot) - grown;
-            // a new block is read off the stack: its table entry may be another CTA's to write
-            const int block = p >= have && grown > 0 ? __ldcg(a.stack + free0 + S - 1 - (grow0[slot] + p - have))
-                                                      : a.table[(size_t)slot * a.max_blocks + p];
-            if (paged_block_ok(block, a.n_blocks)) at = block * br + pos % br;
+    const bool go = !bad && !full;  // else nothing changes, and no row takes part in what follows
+    for (int i = gtid; i <= n; i += step) a.row0[i] = go ? row0[i] : 0;
+    if (go) {
+        auto want_of = [&](int i) { return (int)paged_div_up((unsigned)a.kv_len[i] + (unsigned)a.n_new[i], a.by_rows); };
+        for (int i = gtid; i < n; i += step) a.seq_blocks[i] = want_of(i);
+        for (int e = gtid; e < S; e += step) {
+            const int i = find_owner(shrink0, n, a.top_step, e);
+            int32_t* entry = a.table + (size_t)i * a.max_blocks + want_of(i) + (e - shrink0[i]);
+            a.stack[free0 + S - 1 - e] = *entry;
+            *entry = 0;
         }
-        a.row_slot[r] = slot;
-        a.row_pos[r] = pos;
-        a.slot_map[r] = at;
+        if (S > 0) everyone();  // the pushes are on the stack
+        for (int e = gtid; e < G; e += step) {
+            const int i = find_owner(grow0, n, a.top_step, e);  // its new blocks end at want_of(i)
+            a.table[(size_t)i * a.max_blocks + want_of(i) + (e - grow0[i + 1])] = __ldcg(a.stack + free0 + S - 1 - e);
+        }
+    }
+    if (write_rows) {
+        if (go && G > 0) everyone();  // the table is written
+        const int rows = go ? (int)total.rows : 0;
+        for (int r = gtid; r < a.n_rows; r += step) {
+            if (r < rows) {
+                const int i = find_owner(row0, n, a.top_step, r);
+                write_row(a, r, i, row0[i], a.kv_len[i]);
+            } else {
+                a.row_slot[r] = a.row_pos[r] = a.slot_map[r] = -1;
+            }
+        }
+    }
+}
+
+constexpr int kRowThreads = 256;
+
+// A row a thread; the sequences' first rows are searched in shared memory.
+__global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const PlanArgs a) {
+    extern __shared__ int plan_smem[];
+    pdl_trigger();
+    pdl_wait();
+    const int n = a.n_seqs;
+    for (int i = threadIdx.x; i <= n; i += kRowThreads) plan_smem[i] = __ldcg(a.row0 + i);
+    __syncthreads();
+    const int rows = plan_smem[n];  // 0 when the plan did not go through
+    for (int r = blockIdx.x * kRowThreads + threadIdx.x; r < a.n_rows; r += gridDim.x * kRowThreads) {
+        if (r < rows) {
+            const int i = find_owner(plan_smem, n, a.top_step, r);
+            write_row(a, r, i, plan_smem[i], a.kv_len[i]);
+        } else {
+            a.row_slot[r] = a.row_pos[r] = a.slot_map[r] = -1;
+        }
     }
 }
 
@@ -334,13 +361,24 @@ extern "C" int b200_paged_plan(b200_ctx* ctx, const b200_paged_cache* c, const b
     if (ctx->device < 0) B200_FAIL(ctx, B200_CUDA_ERROR, "b200_paged_plan: the context has no device");
     DeviceScope dev;
     CUDA_TRY(ctx, dev.enter(ctx->device));
+    int top_step = 1;
+    while (top_step * 2 < c->n_seqs) top_step *= 2;
     const PlanArgs a{c->block_table, c->seq_blocks, c->free_blocks, c->free_count, kv_len, n_new, r->seq_row0, r->row_slot, r->row_pos, r->slot_map,
-                     r->status, c->n_seqs, c->n_blocks, c->max_blocks, c->block_rows, r->n_rows};
-    static SmemLimit limit;
-    const size_t smem = 3 * sizeof(int) * ((size_t)c->n_seqs + 1);
+                     r->status, c->n_seqs, c->n_blocks, c->max_blocks, c->block_rows, r->n_rows, paged_divisor(c->block_rows), top_step};
+    static SmemLimit limit, rows_limit;
+    const size_t scan = sizeof(int) * ((size_t)c->n_seqs + 1);
     CUDA_TRY(ctx, limit.raise(paged_plan_kernel, ctx->device, 3 * sizeof(int) * (kPlanMaxSeqs + 1)));
-    const int ctas = 8;
-    launch_cluster(paged_plan_kernel, ctas, dim3(ctas), dim3(kPlanThreads), smem, ctx->stream, a);
+    const bool apart = r->n_rows > 2 * kPlanThreads;
+    // sequences and blocks enough for four a thread: a cluster (2000 sequences with 64000 rows, both calls of a round: 17.3 against
+    // 21.8 us with one CTA)
+    const int ctas = c->n_seqs + r->n_rows / c->block_rows > 4 * kPlanThreads ? 8 : 1;
+    launch_cluster(paged_plan_kernel, ctas, dim3(ctas), dim3(kPlanThreads), 3 * scan, ctx->stream, a, apart ? 0 : 1);
+    if (apart) {
+        LAUNCH_CHECK(ctx);
+        CUDA_TRY(ctx, rows_limit.raise(paged_rows_kernel, ctx->device, sizeof(int) * (kPlanMaxSeqs + 1)));
+        const int most = 2 * ctx->sm_count, blocks = ceil_div(r->n_rows, kRowThreads);
+        launch_pdl(paged_rows_kernel, dim3(blocks < most ? blocks : most), dim3(kRowThreads), scan, ctx->stream, a);
+    }
     LAUNCH_CHECK(ctx);
     return B200_OK;
 }

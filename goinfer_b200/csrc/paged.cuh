@@ -18,6 +18,12 @@ __host__ __device__ inline int paged_visible(int pos, int block_rows, int max_bl
     return (b < max_blocks ? b : max_blocks - 1) + 1;
 }
 
+// Division by block_rows (16 d, d <= 16) of x < 2^31 without the instruction sequence of a division: x / 16d = (x >> 4) / d,
+// and y / d = y * ceil(2^31 / d) >> 31 for y < 2^27, because y times what the ceiling adds (below 1) stays below 2^31 / d.
+inline unsigned paged_divisor(int block_rows) { return (unsigned)(((1ull << 31) + (unsigned)block_rows / 16 - 1) / ((unsigned)block_rows / 16)); }
+__host__ __device__ inline unsigned paged_div(unsigned x, unsigned divisor) { return (unsigned)(((unsigned long long)(x >> 4) * divisor) >> 31); }
+__host__ __device__ inline unsigned paged_div_up(unsigned x, unsigned divisor) { return x == 0 ? 0 : paged_div(x - 1, divisor) + 1; }
+
 // Halves in front of row 0 of a block's tile of one kv head. 64-bit: a pool passes 2^31 elements at 4 GB.
 __host__ __device__ inline size_t paged_tile(int block, int kvh, int n_kv, int block_rows, int hd) {
     return ((size_t)block * n_kv + kvh) * block_rows * hd;
@@ -59,7 +65,7 @@ inline void launch_cluster(void (*kernel)(KArgs...), int cluster, dim3 grid, dim
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
     cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);  // an error surfaces in LAUNCH_CHECK's cudaGetLastError
 }
 

@@ -4,9 +4,10 @@
 // over the keys j <= position of the listed blocks. One pass with a running maximum and sum; a row without a key gives 0.
 //
 // One cluster of CTAs per (row, kv head) shares out the listed blocks; each CTA's four warps walk 16-key tiles of their own
-// through private cp.async rings, and the warps' and the CTAs' states (accumulators, maximum, sum) are joined in shared
-// memory, the CTAs' through distributed shared memory: nothing is parked in global memory, so the call needs no workspace
-// and calls on several streams share nothing.
+// through private cp.async rings, and the warps' states (accumulators, maximum, sum) are joined in shared memory. Each CTA of
+// the cluster owns a share of the outputs: the others store their states of it into the owner's shared memory, and behind one
+// cluster barrier the owner joins them. Nothing is parked in global memory, so the call needs no workspace and calls on
+// several streams share nothing.
 //
 // Products run on mma.sync m16n8k16 over the fp16 cache with fp32 accumulation; f32 queries and weights are split into
 // fp16 hi + lo parts (x = hi + lo to 2^-22), so the result keeps fp32 accuracy. S[head][key] = Q K^T takes the group's
@@ -18,8 +19,9 @@
 
 namespace {
 
-constexpr int kAttWarps = 4, kAttThreads = 32 * kAttWarps, kAttStages = 3;
+constexpr int kAttWarps = 4, kAttThreads = 32 * kAttWarps, kAttStages = 2;
 constexpr int kAttMaxList = 2048;
+constexpr int kAttMaxCluster = 8;
 
 __device__ __forceinline__ void ldm4(unsigned addr, unsigned (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -48,6 +50,10 @@ template <int HD>
 struct AttendShape {
     static constexpr int KS = HD / 16, CPR = HD / 8, ROWB = HD * 2, TILE = 16 * ROWB, CPL = 16 * CPR / 32;
     static constexpr size_t ring = (size_t)kAttWarps * kAttStages * 2 * TILE;
+    // what the cluster's CTAs send this one: its share of the outputs of each, then their maxima and sums
+    static constexpr size_t inbox = 8 * HD + 2 * kAttMaxCluster * 8;
+    static constexpr size_t smem(int n_select) { return ring + sizeof(float) * inbox + sizeof(int2) * (size_t)n_select; }
+    static constexpr int ACC = HD + 4;  // floats between heads in the warps' states: the fragments' stores meet no bank twice
 };
 
 template <int HD>
@@ -57,50 +63,101 @@ __global__ void __launch_bounds__(kAttThreads) paged_attend_kernel(const b200_pa
                                                                    float* __restrict__ out, size_t ldo) {
     using S = AttendShape<HD>;
     constexpr int KS = S::KS, CPR = S::CPR, ROWB = S::ROWB, TILE = S::TILE, CPL = S::CPL;
-    extern __shared__ __align__(128) uint8_t att_smem[];  // rings, then the list: page and first key of each block
-    int2* list = reinterpret_cast<int2*>(att_smem + S::ring);
+    extern __shared__ __align__(128) uint8_t att_smem[];  // rings, inbox, then the list: page and first key of each block
+    float* inbox = reinterpret_cast<float*>(att_smem + S::ring);
+    int2* list = reinterpret_cast<int2*>(inbox + S::inbox);
     __shared__ int s_count[kAttWarps];
     const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
     const int r = blockIdx.x / ctas, kvh = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
+    // the row's place, the first entries of its list and its queries are fetched together
+    const int32_t* lp = sel + ((size_t)r * c.n_kv_heads + kvh) * n_select;
     const int slot = row_slot[r], pos = row_pos[r], br = c.block_rows;
+    int entry = tid < n_select ? lp[tid] : -1;
+    float2 qa[KS], qb[KS];
+    {
+        const float* qp = q + (size_t)r * ldq + (size_t)(kvh * G + (gid < G ? gid : 0)) * HD;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            qa[ks] = *reinterpret_cast<const float2*>(qp + 16 * ks + 2 * tig);
+            qb[ks] = *reinterpret_cast<const float2*>(qp + 16 * ks + 8 + 2 * tig);
+        }
+    }
     if (!paged_row_ok(slot, pos, c.n_seqs)) return;  // the whole cluster leaves; the row's output stays as it was
+    if (ctas > 1) cluster_arrive();
 
     // the listed blocks that hold a key the row sees, in the list's order
     const int have = paged_visible(pos, br, c.max_blocks);
     const int n_keys = min(pos, have * br - 1) + 1;
     const int32_t* tbl = c.block_table + (size_t)slot * c.max_blocks;
-    const int32_t* lp = sel + ((size_t)r * c.n_kv_heads + kvh) * n_select;
     int n_list = 0;
     for (int i0 = 0; i0 < n_select; i0 += kAttThreads) {
-        const int b = i0 + tid < n_select ? lp[i0 + tid] : -1;
+        const int b = entry;
+        if (i0 + kAttThreads < n_select) entry = i0 + kAttThreads + tid < n_select ? lp[i0 + kAttThreads + tid] : -1;
         const int page = b >= 0 && b < have ? tbl[b] : 0;
         const bool in = paged_block_ok(page, c.n_blocks);
         const unsigned ballot = __ballot_sync(0xffffffffu, in);
+        if (i0 > 0) __syncthreads();  // the counts of the round before have been read
         if (lane == 0) s_count[warp] = __popc(ballot);
         __syncthreads();
         int at = n_list + __popc(ballot & ((1u << lane) - 1u));
+#pragma unroll
         for (int w = 0; w < kAttWarps; w++) {
             if (w < warp) at += s_count[w];
             n_list += s_count[w];
         }
         if (in) list[at] = make_int2(page, b * br);
-        __syncthreads();
     }
+    __syncthreads();
+
+    // this warp's tiles: t0 + warp, t0 + warp + 4, ... of the cluster's n_list * (br / 16); (e, sub): block and tile in it
+    const int tpb = br >> 4, tiles = n_list * tpb;
+    const int t0 = tiles * rank / ctas, t1 = tiles * (rank + 1) / ctas;
+    const int n_mine = t0 + warp < t1 ? (t1 - t0 - warp + kAttWarps - 1) / kAttWarps : 0;
+    const unsigned ring = (unsigned)__cvta_generic_to_shared(att_smem) + (unsigned)(warp * kAttStages * 2 * TILE);
+    const int de = kAttWarps / tpb, dsub = kAttWarps - de * tpb;
+    struct Place {
+        int e, sub;
+    };
+    auto advance = [&](Place& p) {
+        p.e += de;
+        p.sub += dsub;
+        if (p.sub >= tpb) { p.sub -= tpb; p.e++; }
+    };
+    Place next{(t0 + warp) / tpb, 0};
+    next.sub = t0 + warp - next.e * tpb;
+    Place now = next;
+    const size_t copy_at = (size_t)kvh * br * HD * 2 + 16 * lane;  // of a lane's first 16 bytes in a block
+    const size_t block_bytes = (size_t)c.n_kv_heads * br * HD * 2;
+    auto issue = [&](int it) {
+        if (it < n_mine) {
+            const int2 b = list[next.e];
+            const int keys = n_keys - (b.y + 16 * next.sub);  // of the tile's sixteen, the ones that the row sees
+            const size_t off = (size_t)b.x * block_bytes + copy_at + (size_t)(next.sub * TILE);
+            const uint8_t *ks = static_cast<const uint8_t*>(c.k_pool) + off, *vs = static_cast<const uint8_t*>(c.v_pool) + off;
+            const unsigned dst = ring + (unsigned)((it % kAttStages) * 2 * TILE);
+#pragma unroll
+            for (int i = 0; i < CPL; i++) {
+                const int ci = lane + 32 * i, row = ci / CPR, ch = ci % CPR;
+                const unsigned d = (unsigned)(row * ROWB + ((ch ^ (row & 7)) << 4));
+                copy16(dst + d, ks + i * 512, row < keys);
+                copy16(dst + TILE + d, vs + i * 512, row < keys);
+            }
+            advance(next);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int s = 0; s < kAttStages - 1; s++) issue(s);
 
     // the head's largest |q| is brought to [1, 2) by a power of two, which the scale gives back: neither a query beyond fp16's
     // range nor one among its subnormals loses anything
     unsigned qh0[KS], qh2[KS], ql0[KS], ql2[KS];
     {
-        const float* qp = q + (size_t)r * ldq + (size_t)(kvh * G + (gid < G ? gid : 0)) * HD;
-        float2 qa[KS], qb[KS];
         float most = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            qa[ks] = *reinterpret_cast<const float2*>(qp + 16 * ks + 2 * tig);
-            qb[ks] = *reinterpret_cast<const float2*>(qp + 16 * ks + 8 + 2 * tig);
+        for (int ks = 0; ks < KS; ks++)
             most = fmaxf(fmaxf(most, fmaxf(fabsf(qa[ks].x), fabsf(qa[ks].y))), fmaxf(fabsf(qb[ks].x), fabsf(qb[ks].y)));
-        }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const int e = (int)(__float_as_uint(most) >> 23) - 127;
@@ -118,47 +175,15 @@ __global__ void __launch_bounds__(kAttThreads) paged_attend_kernel(const b200_pa
     for (int mt = 0; mt < KS; mt++) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
 
-    // this warp's tiles: t0 + warp, t0 + warp + 4, ... of the cluster's n_list * (br / 16)
-    const int tpb = br >> 4, tiles = n_list * tpb;
-    const int t0 = (int)((long long)tiles * rank / ctas), t1 = (int)((long long)tiles * (rank + 1) / ctas);
-    const int n_mine = t0 + warp < t1 ? (t1 - t0 - warp + kAttWarps - 1) / kAttWarps : 0;
-    const unsigned ring = (unsigned)__cvta_generic_to_shared(att_smem) + (unsigned)(warp * kAttStages * 2 * TILE);
-    auto first_key = [&](int it, int& page, int& row0) {
-        const int t = t0 + warp + kAttWarps * it, e = t / tpb;
-        row0 = (t - e * tpb) << 4;
-        page = list[e].x;
-        return list[e].y + row0;
-    };
-    auto issue = [&](int it) {
-        if (it < n_mine) {
-            int page, row0;
-            const int key0 = first_key(it, page, row0);
-            const size_t off = paged_tile(page, kvh, c.n_kv_heads, br, HD) + (size_t)row0 * HD;
-            const uint8_t* ks = reinterpret_cast<const uint8_t*>(static_cast<const __half*>(c.k_pool) + off);
-            const uint8_t* vs = reinterpret_cast<const uint8_t*>(static_cast<const __half*>(c.v_pool) + off);
-            const unsigned dst = ring + (unsigned)((it % kAttStages) * 2 * TILE);
-#pragma unroll
-            for (int i = 0; i < CPL; i++) {
-                const int ci = lane + 32 * i, row = ci / CPR, ch = ci % CPR;
-                const unsigned d = (unsigned)(row * ROWB + ((ch ^ (row & 7)) << 4));
-                const bool there = key0 + row < n_keys;
-                copy16(dst + d, ks + ci * 16, there);
-                copy16(dst + TILE + d, vs + ci * 16, there);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int s = 0; s < kAttStages - 1; s++) issue(s);
-
+    const float inv_cap = cap != 0.f ? 1.f / cap : 0.f;
     const int lrow = (lane & 7) + ((lane >> 4) << 3), lsel = (lane >> 3) & 1;
     for (int it = 0; it < n_mine; it++) {
         issue(it + kAttStages - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(kAttStages - 1) : "memory");
         __syncwarp();
         const unsigned kb = ring + (unsigned)((it % kAttStages) * 2 * TILE), vb = kb + TILE;
-        int page, row0;
-        const int key0 = first_key(it, page, row0);
+        const int key0 = list[now.e].y + 16 * now.sub;
+        advance(now);
         float s0h[4] = {0, 0, 0, 0}, s0l[4] = {0, 0, 0, 0}, s1h[4] = {0, 0, 0, 0}, s1l[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
@@ -175,7 +200,7 @@ __global__ void __launch_bounds__(kAttThreads) paged_attend_kernel(const b200_pa
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             x[i] *= scale;  // this lane's scores are all of head gid
-            if (cap != 0.f) x[i] = cap * tanhf(x[i] / cap);
+            if (cap != 0.f) x[i] = cap * tanhf(x[i] * inv_cap);
             if (kk[i] >= n_keys) x[i] = -INFINITY;
             mx = fmaxf(mx, x[i]);
         }
@@ -214,58 +239,69 @@ __global__ void __launch_bounds__(kAttThreads) paged_attend_kernel(const b200_pa
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    // join the warps (in the rings' room): acc[warp][head][dim], then maximum and sum [warp][head]; the CTA's own state
-    // lies behind them, where the cluster reads it
+    // join the warps (in the rings' room): acc[warp][head][dim], then maximum and sum [warp][head]
     float* acc = reinterpret_cast<float*>(att_smem);
-    float* sm_m = acc + kAttWarps * G * HD;
-    float* sm_l = sm_m + kAttWarps * G;
-    float* cta = sm_l + kAttWarps * G;  // [G][HD], [G] maximum, [G] sum
+    float* sm_m = acc + kAttWarps * 8 * S::ACC;
+    float* sm_l = sm_m + kAttWarps * 8;
     if (tig == 0 && gid < G) {
-        sm_m[warp * G + gid] = m_run;
-        sm_l[warp * G + gid] = l_run;
+        sm_m[warp * 8 + gid] = m_run;
+        sm_l[warp * 8 + gid] = l_run;
     }
 #pragma unroll
     for (int mt = 0; mt < KS; mt++) {
         const int h0 = 2 * tig, h1 = h0 + 1, d0 = 16 * mt + gid;
-        if (h0 < G) { acc[(warp * G + h0) * HD + d0] = o[mt][0]; acc[(warp * G + h0) * HD + d0 + 8] = o[mt][2]; }
-        if (h1 < G) { acc[(warp * G + h1) * HD + d0] = o[mt][1]; acc[(warp * G + h1) * HD + d0 + 8] = o[mt][3]; }
+        if (h0 < G) { acc[(warp * 8 + h0) * S::ACC + d0] = o[mt][0]; acc[(warp * 8 + h0) * S::ACC + d0 + 8] = o[mt][2]; }
+        if (h1 < G) { acc[(warp * 8 + h1) * S::ACC + d0] = o[mt][1]; acc[(warp * 8 + h1) * S::ACC + d0 + 8] = o[mt][3]; }
     }
     __syncthreads();
-    for (int idx = tid; idx < G * HD; idx += kAttThreads) {
+    if (ctas > 1) cluster_wait();  // the CTAs have started: their shared memory may be written
+    // value idx of the CTA's state goes to the CTA that owns it (share = values a CTA owns), maxima and sums to all
+    const int values = G * HD, share = values / ctas;
+    float* out_row = out + (size_t)r * ldo + (size_t)kvh * values;
+    for (int idx = tid; idx < values; idx += kAttThreads) {
         const int g = idx / HD, e = idx % HD;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kAttWarps; w++) M = fmaxf(M, sm_m[w * G + g]);
+        for (int w = 0; w < kAttWarps; w++) M = fmaxf(M, sm_m[w * 8 + g]);
         const float ref = M == -INFINITY ? 0.f : M;
         float tot = 0.f, l = 0.f;
 #pragma unroll
         for (int w = 0; w < kAttWarps; w++) {
-            const float f = __expf(sm_m[w * G + g] - ref);
-            tot += acc[(w * G + g) * HD + e] * f;
-            l += sm_l[w * G + g] * f;
+            const float f = __expf(sm_m[w * 8 + g] - ref);
+            tot = fmaf(acc[(w * 8 + g) * S::ACC + e], f, tot);
+            l = fmaf(sm_l[w * 8 + g], f, l);
         }
-        cta[idx] = tot;
-        if (e == 0) {
-            cta[G * HD + g] = M;
-            cta[G * HD + G + g] = l;
+        if (ctas == 1) {
+            out_row[idx] = l > 0.f || l != l ? tot / l : 0.f;
+        } else {
+            cluster_store(cluster_addr(inbox + rank * share + idx % share, idx / share), tot);
+            if (e < ctas) {
+                cluster_store(cluster_addr(inbox + 8 * HD + rank * 8 + g, e), M);
+                cluster_store(cluster_addr(inbox + 8 * HD + (kAttMaxCluster + rank) * 8 + g, e), l);
+            }
         }
     }
-    cluster_sync();
-    // every CTA joins its share of the outputs over all CTAs, in their order
-    for (int idx = rank * kAttThreads + tid; idx < G * HD; idx += ctas * kAttThreads) {
-        const int g = idx / HD;
+    if (ctas == 1) return;
+    cluster_sync();  // what the CTAs sent has arrived
+    for (int i = tid; i < share; i += kAttThreads) {
+        const int idx = rank * share + i, g = idx / HD;
+        const float* ms = inbox + 8 * HD + g;
         float M = -INFINITY;
-        for (int w = 0; w < ctas; w++) M = fmaxf(M, cluster_load_f32(cluster_addr(cta + G * HD + g, w)));
+#pragma unroll
+        for (int w = 0; w < kAttMaxCluster; w++)
+            if (w < ctas) M = fmaxf(M, ms[w * 8]);
         const float ref = M == -INFINITY ? 0.f : M;
         float tot = 0.f, l = 0.f;
-        for (int w = 0; w < ctas; w++) {
-            const float f = __expf(cluster_load_f32(cluster_addr(cta + G * HD + g, w)) - ref);
-            tot += cluster_load_f32(cluster_addr(cta + idx, w)) * f;
-            l += cluster_load_f32(cluster_addr(cta + G * HD + G + g, w)) * f;
+#pragma unroll
+        for (int w = 0; w < kAttMaxCluster; w++) {
+            if (w < ctas) {
+                const float f = __expf(ms[w * 8] - ref);
+                tot = fmaf(inbox[w * share + i], f, tot);
+                l = fmaf(ms[(kAttMaxCluster + w) * 8], f, l);
+            }
         }
-        out[(size_t)r * ldo + (size_t)kvh * G * HD + idx] = l > 0.f || l != l ? tot / l : 0.f;
+        out_row[idx] = l > 0.f || l != l ? tot / l : 0.f;
     }
-    cluster_sync();  // no CTA leaves while another reads its state
 }
 
 }  // namespace
@@ -293,17 +329,21 @@ extern "C" int b200_paged_attend(b200_ctx* ctx, const b200_paged_cache* c, const
     CUDA_TRY(ctx, dev.enter(ctx->device));
     const int G = n_heads / c->n_kv_heads, tiles = n_select * (c->block_rows / 16);
     const float s = scale != 0.f ? scale : 1.0f / sqrtf((float)c->head_dim);
+    // As many CTAs a (row, kv head) as fit the GPU at once (two an SM at head_dim 128, four at 64), each with a tile a warp at
+    // least: one more wave costs more than the shorter share saves. Rows x kv heads x tiles, in us with 1, 2, 4, 8 CTAs:
+    // 8 x 64: 13.0, 9.4, 6.9, 5.9; 64 x 64: 13.4, 10.0, 8.5, 12.9; 128 x 64: 16.9, 16.5, 20.6, 29.9; 384 x 66: 45, 49, 60, 87.
     int ctas = 1;
-    while (ctas < 8 && (long long)r->n_rows * c->n_kv_heads * ctas < 4 * ctx->sm_count && tiles / ctas > 8) ctas *= 2;
+    const int at_once = (c->head_dim == 128 ? 2 : 4) * ctx->sm_count;
+    while (ctas < kAttMaxCluster && 2ll * r->n_rows * c->n_kv_heads * ctas <= at_once && tiles >= 2 * kAttWarps * ctas) ctas *= 2;
     const dim3 grid((unsigned)(r->n_rows * ctas), c->n_kv_heads);
     static SmemLimit limit[2];
     if (c->head_dim == 128) {
-        CUDA_TRY(ctx, limit[1].raise(paged_attend_kernel<128>, ctx->device, AttendShape<128>::ring + sizeof(int2) * kAttMaxList));
-        launch_cluster(paged_attend_kernel<128>, ctas, grid, dim3(kAttThreads), AttendShape<128>::ring + sizeof(int2) * n_select, ctx->stream, *c, r->row_slot,
+        CUDA_TRY(ctx, limit[1].raise(paged_attend_kernel<128>, ctx->device, AttendShape<128>::smem(kAttMaxList)));
+        launch_cluster(paged_attend_kernel<128>, ctas, grid, dim3(kAttThreads), AttendShape<128>::smem(n_select), ctx->stream, *c, r->row_slot,
                        r->row_pos, q, (size_t)ldq, G, s, softcap, sel, n_select, out, (size_t)ldo);
     } else {
-        CUDA_TRY(ctx, limit[0].raise(paged_attend_kernel<64>, ctx->device, AttendShape<64>::ring + sizeof(int2) * kAttMaxList));
-        launch_cluster(paged_attend_kernel<64>, ctas, grid, dim3(kAttThreads), AttendShape<64>::ring + sizeof(int2) * n_select, ctx->stream, *c, r->row_slot,
+        CUDA_TRY(ctx, limit[0].raise(paged_attend_kernel<64>, ctx->device, AttendShape<64>::smem(kAttMaxList)));
+        launch_cluster(paged_attend_kernel<64>, ctas, grid, dim3(kAttThreads), AttendShape<64>::smem(n_select), ctx->stream, *c, r->row_slot,
                        r->row_pos, q, (size_t)ldq, G, s, softcap, sel, n_select, out, (size_t)ldo);
     }
     LAUNCH_CHECK(ctx);

@@ -53,11 +53,20 @@ int main() {
     assert(paged_visible(0, 16, 8) == 1 && paged_visible(15, 16, 8) == 1 && paged_visible(16, 16, 8) == 2);
     assert(paged_visible(127, 16, 8) == 8 && paged_visible(128, 16, 8) == 8 && paged_visible(INT_MAX, 16, 8) == 8 && paged_visible(5, 256, 1) == 1);
     assert(paged_tile(1 << 20, 7, 8, 64, 128) == (((size_t)1 << 23) + 7) * 64 * 128);
+    for (int br = 16; br <= 256; br += 16) {
+        const unsigned d = paged_divisor(br);
+        for (unsigned k = 0; k < 5000000; k++) {
+            const unsigned x = k < 100000 ? k : k % 3 == 0 ? (k * 2654435761u) >> 1 : k % 3 == 1 ? (k * 429u) / br * br : (k * 429u) / br * br + br - 1;
+            if (x >= 0x80000000u) continue;
+            assert(paged_div(x, d) == x / br && paged_div_up(x, d) == (x + (unsigned)br - 1) / br);
+        }
+        for (unsigned x = 0x7fffffffu; x > 0x7fffffffu - 100000; x--) assert(paged_div(x, d) == x / br && paged_div_up(x, d) == (x + (unsigned)br - 1) / br);
+    }
     return 0;
 }
 """)
     exe = tmp_path / "rules"
-    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, "goinfer_b200", "csrc"), "-I", "/usr/local/cuda/include", str(src), "-o", str(exe)], check=True)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", os.path.join(ROOT, "goinfer_b200", "csrc"), "-I", "/usr/local/cuda/include", str(src), "-o", str(exe)], check=True)
     subprocess.run([str(exe)], check=True)
 
 
