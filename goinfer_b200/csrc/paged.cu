@@ -64,7 +64,8 @@ __device__ __forceinline__ Sums warp_inclusive(Sums v, int lane) {
 }
 
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs a, int write_rows) {
-    pdl_trigger();  // the rows' kernel waits for this one's end
+    pdl_trigger();
+    pdl_wait();
     extern __shared__ int plan_smem[];
     int* row0 = plan_smem;                    // [n + 1] scan of new rows
     int* grow0 = row0 + a.n_seqs + 1;         // [n + 1] scan of blocks taken
@@ -235,6 +236,8 @@ template <int HD>
 __global__ void __launch_bounds__(32 * kAppendMaxWarps) paged_append_kernel(const b200_paged_cache c, const int32_t* __restrict__ slot_map, int n_rows,
                                                                             const float* __restrict__ k, size_t ldk, const float* __restrict__ v,
                                                                             size_t ldv, int rows_per_cta, int parts) {
+    pdl_trigger();
+    pdl_wait();
     constexpr int LPR = HD / 4, RPW = 32 / LPR, U = 4;  // lanes a row, rows a warp at a time, loads in flight
     __shared__ Bounds4 joined[kAppendMaxWarps][LPR];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, br = c.block_rows;
@@ -405,7 +408,8 @@ extern "C" int b200_paged_append(b200_ctx* ctx, const b200_paged_cache* c, const
     const int parts = c->n_kv_heads < warps ? warps / c->n_kv_heads : 1;
     const int threads = 32 * (c->n_kv_heads < warps ? c->n_kv_heads * parts : warps);
     auto kernel = c->head_dim == 128 ? paged_append_kernel<128> : paged_append_kernel<64>;
-    kernel<<<ceil_div(r->n_rows, rows), threads, 0, ctx->stream>>>(*c, r->slot_map, r->n_rows, k, (size_t)ldk, v, (size_t)ldv, rows, parts);
+    launch_cluster(kernel, 1, dim3(ceil_div(r->n_rows, rows)), dim3(threads), 0, ctx->stream, *c, r->slot_map, r->n_rows, k, (size_t)ldk, v, (size_t)ldv, rows,
+                   parts);
     LAUNCH_CHECK(ctx);
     return B200_OK;
 }

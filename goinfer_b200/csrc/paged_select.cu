@@ -156,6 +156,7 @@ template <int HD>
 __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200_paged_cache c, const int32_t* __restrict__ row_slot,
                                                                    const int32_t* __restrict__ row_pos, const float* __restrict__ q, size_t ldq, int G,
                                                                    int n_first, int n_recent, int n_select, int max_chunk, int32_t* __restrict__ sel) {
+    pdl_wait();
     // the CTA's blocks: s~ (with many blocks in doubt, words of their keys), a bit for those that are in, one for those in doubt
     extern __shared__ __align__(16) float sel_score[];
     unsigned* in_bits = reinterpret_cast<unsigned*>(sel_score + max_chunk);
@@ -307,6 +308,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
                 if (tig == 0 && b < own) sel_score[b] = ok ? s : -INFINITY;
             }
         }
+        pdl_trigger();
         err_bits = __reduce_max_sync(0xffffffffu, err_bits);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {

@@ -2,6 +2,7 @@
 Python views (nothing is queued by a refused call)."""
 import ctypes as C
 import os
+import re
 import subprocess
 
 import pytest
@@ -68,6 +69,20 @@ int main() {
     exe = tmp_path / "rules"
     subprocess.run(["g++", "-O2", "-std=c++17", "-I", os.path.join(ROOT, "goinfer_b200", "csrc"), "-I", "/usr/local/cuda/include", str(src), "-o", str(exe)], check=True)
     subprocess.run([str(exe)], check=True)
+
+
+def test_every_kernel_waits_for_the_one_before_it():
+    """The paged kernels start while the kernel ahead of them still runs: each must wait before its first statement that reads."""
+    n = 0
+    for name in ("paged.cu", "paged_select.cu", "paged_attend.cu"):
+        text = re.sub(r"//[^\n]*", "", open(os.path.join(ROOT, "goinfer_b200", "csrc", name)).read())
+        assert "<<<" not in text
+        for m in re.finditer(r"__global__[^{]*\{", text):
+            n += 1
+            body = text[m.end():].lstrip()
+            body = re.sub(r"^extern __shared__[^;]*;\s*", "", body)
+            assert re.match(r"(pdl_trigger\(\);\s*)?pdl_wait\(\);", body), m.group(0)
+    assert n == 5
 
 
 A = 1 << 20  # an aligned address that no call reads
