@@ -88,10 +88,11 @@ __device__ __forceinline__ void find_bin(const unsigned* hist, int ctas, int nee
     if (ctas == 1) {
         h = *reinterpret_cast<const uint4*>(hist + first);
     } else {
-        for (int w = 0; w < ctas; w++) {
-            const uint4 t = cluster_load_u32x4(cluster_addr(hist + first, w));
-            h.x += t.x; h.y += t.y; h.z += t.z; h.w += t.w;
-        }
+        uint4 t[kSelMaxCluster];
+#pragma unroll
+        for (int w = 0; w < kSelMaxCluster; w++) t[w] = w < ctas ? cluster_load_u32x4(cluster_addr(hist + first, w)) : h;
+#pragma unroll
+        for (int w = 0; w < kSelMaxCluster; w++) { h.x += t[w].x; h.y += t[w].y; h.z += t[w].z; h.w += t[w].w; }
     }
     const int count[4] = {(int)h.w, (int)h.z, (int)h.y, (int)h.x};
     const int mine = count[0] + count[1] + count[2] + count[3];
@@ -176,6 +177,11 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
     const int ctas = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = blockIdx.x / ctas, kvh = blockIdx.y;
     const int slot = row_slot[r], pos = row_pos[r];
+    const float* qr = q + (size_t)r * ldq + (size_t)kvh * G * HD;
+    float4 q_ahead[8 * HD / (4 * kSelThreads)];  // on its way beside the row's place
+#pragma unroll
+    for (int i = 0; i < 8 * HD / (4 * kSelThreads); i++)
+        q_ahead[i] = tid + i * kSelThreads < G * HD / 4 ? reinterpret_cast<const float4*>(qr)[tid + i * kSelThreads] : make_float4(0.f, 0.f, 0.f, 0.f);
     if (!paged_row_ok(slot, pos, c.n_seqs)) return;  // the whole cluster leaves; the row's list stays as it was
     int32_t* out = sel + ((size_t)r * c.n_kv_heads + kvh) * n_select;
     const int have = paged_visible(pos, c.block_rows, c.max_blocks);
@@ -187,7 +193,6 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
     const int n = have - n_first - n_recent;  // the middle blocks n_first .. n_first + n - 1
     const int m = n_select - n_first - n_recent;
     const int32_t* tbl = c.block_table + (size_t)slot * c.max_blocks + n_first;  // of this CTA's blocks from below on
-    const float* qr = q + (size_t)r * ldq + (size_t)kvh * G * HD;
     if (rank == 0) {
         for (int i = tid; i < n_first; i += kSelThreads) out[i] = i;
         for (int i = tid; i < n_recent; i += kSelThreads) out[n_select - n_recent + i] = have - n_recent + i;
@@ -211,7 +216,8 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
         int b0 = 16 * warp;
         auto page_of = [&](int b) { return b < own ? tbl[b] : 0; };
         int page0 = page_of(b0 + gid), page1 = page_of(b0 + 8 + gid);
-        for (int i = tid; i < G * HD / 4; i += kSelThreads) reinterpret_cast<float4*>(&sq[0][0])[i] = reinterpret_cast<const float4*>(qr)[i];
+#pragma unroll
+        for (int i = 0; i < 8 * HD / (4 * kSelThreads); i++) reinterpret_cast<float4*>(&sq[0][0])[tid + i * kSelThreads] = q_ahead[i];
         __syncthreads();
         // the columns' powers of two against the group's largest; columns past the group repeat its first head
         float f0, f1;
