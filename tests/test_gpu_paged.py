@@ -178,6 +178,35 @@ def test_append_stores_rows_and_bounds(ops, kv, hd, br, bounded):
             np.testing.assert_array_equal(got.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("kv,hd,br,news", [(2, 64, 16, (901, 0, 777)), (8, 128, 32, (300, 13, 500)), (1, 128, 64, (2049, 1, 2700)), (3, 64, 16, (5000, 1, 17))])
+def test_append_of_many_rows(ops, kv, hd, br, news):
+    """Prompts: a CTA looks for runs among several rows, runs begin and end anywhere among them."""
+    rng = np.random.default_rng(br)
+    torch.manual_seed(br)
+    n_blocks = sum(-(-(n + br) // br) for n in news) + 4
+    k_pool = torch.full((n_blocks, kv, br, hd), float("nan"), dtype=torch.float16, device="cuda")
+    v_pool, bounds = torch.zeros_like(k_pool), torch.zeros(n_blocks, kv, 2, hd, dtype=torch.float16, device="cuda")
+    p = Pool(ops, 3, max(news) // br + 2, n_blocks, br, sum(news) + 40, rng, k_pool=k_pool, v_pool=v_pool, key_bounds=bounds)
+    assert p.plan([0, 0, 0], [5, 2, 0]) == 0
+    x = torch.randn(p.n_rows, kv, hd, device="cuda")
+    p.cache.append(p.rows, x, x)
+    assert p.plan([5, 2, 0], news) == 0
+    y = torch.randn(p.n_rows, kv, hd, device="cuda")
+    p.cache.append(p.rows, y, -y)
+    torch.cuda.synchronize()
+    r = 0
+    for s, (first, new, old) in enumerate(zip((5, 2, 0), news, ([0, 5], [5, 7], [7, 7]))):
+        keys = torch.cat((x[old[0]:old[1]], y[r:r + new])).half()
+        r += new
+        for b in range(-(-len(keys) // br)):
+            page, part = int(p.table[s, b]), keys[b * br:(b + 1) * br]
+            assert torch.equal(k_pool[page, :, :len(part)], part.transpose(0, 1))
+            if len(keys) > b * br + (first if b == 0 else 0):  # written to by the second step
+                assert torch.equal(v_pool[page, :, max(0, first - b * br):len(part)], -part[max(0, first - b * br):].transpose(0, 1))
+            assert torch.equal(bounds[page], torch.stack((part.amin(0), part.amax(0)), 1))
+    assert k_pool[0].isnan().all() and bounds[0].eq(0).all()
+
+
 def test_append_leaves_bad_slots_out(ops):
     rng = np.random.default_rng(1)
     pool = torch.zeros(6, 2, 16, 64, dtype=torch.float16, device="cuda")
@@ -429,6 +458,60 @@ def test_attend_offsets_past_32_bits(ops):
     assert torch.equal(bounds[n_blocks - 2, :, 1], pool[n_blocks - 2].amax(1))
     want, worst = _attend_reference(q, pool, pool, table, [0], [4 * br - 1], br, sel, hd ** -0.5, 0.0, out)
     _close(out, want, worst)
+
+
+@pytest.mark.parametrize("rows,kv,G,hd,br,max_blocks,n", [(2, 2, 4, 128, 16, 700, 90), (70, 4, 8, 64, 32, 40, 20)])
+def test_calls_give_the_same_bits_again(ops, rows, kv, G, hd, br, max_blocks, n):
+    rng = np.random.default_rng(rows)
+    torch.manual_seed(rows)
+    n_blocks = 3000
+    k_pool = torch.randn(n_blocks, kv, br, hd, device="cuda").half()
+    v_pool = torch.randn(n_blocks, kv, br, hd, device="cuda").half()
+    bounds = torch.stack((k_pool.amin(2), k_pool.amax(2)), 2).contiguous()
+    table, slot, pos = _context(rng, rows, max_blocks, br, n_blocks)
+    cache, packed = _views(ops, table, slot, pos, br, n_blocks, k_pool, v_pool, bounds)
+    q = torch.randn(rows, kv * G, hd, device="cuda")  # heads as a dimension of their own, in q and in out
+    results = []
+    for _ in range(5):
+        sel = torch.full((rows, kv, n), -1, dtype=torch.int32, device="cuda")
+        out = torch.zeros_like(q)
+        cache.select(packed, q, sel)
+        cache.attend(packed, q, sel, out)
+        results.append((sel, out))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, results[0][0]) and torch.equal(b, results[0][1]) for a, b in results)
+    want, worst = _attend_reference(q.reshape(rows, -1), k_pool, v_pool, table, slot, pos, br, results[0][0].cpu().numpy(), hd ** -0.5, 0.0, out.reshape(rows, -1))
+    _close(out.reshape(rows, -1), want, worst)
+
+
+def test_the_last_sequences_are_retired_by_a_plan_without_rows(ops):
+    p = Pool(ops, 3, 5, 20, 16, 0, np.random.default_rng(0))
+    full = len(p.free)
+    grown = Pool(ops, 3, 5, 20, 16, 90, np.random.default_rng(0))
+    grown.plan([0, 0, 0], [20, 40, 30])
+    for a, b in ((p.d[k], grown.d[k]) for k in p.d):
+        a.copy_(b)
+    p.table, p.blocks, p.free = grown.table.copy(), grown.blocks.copy(), list(grown.free)
+    assert p.plan([20, 0, 30], [0, 0, 0]) == 0 and p.plan([0, 0, 0], [0, 0, 0]) == 0 and len(p.free) == full
+    assert p.plan([0, 0, 0], [1, 0, 0]) == 3  # a row, and no room for it
+
+
+def test_refused_calls_queue_nothing_and_the_device_stays(ops):
+    from goinfer_b200.resident import ResidentError
+    cache, packed = _views(ops, np.ones((2, 4), np.int32), [0, 1], [3, 60], 16, 9, torch.zeros(9, 2, 16, 64, dtype=torch.float16, device="cuda"),
+                           torch.zeros(9, 2, 16, 64, dtype=torch.float16, device="cuda"))
+    q, sel, out = torch.randn(2, 256, device="cuda"), torch.zeros(2, 2, 4, dtype=torch.int32, device="cuda"), torch.full((2, 256), 5.0, device="cuda")
+    before, device = ops.launch_count(), torch.cuda.current_device()
+    for f in (lambda: cache.attend(packed, q, sel, out, softcap=-1.0), lambda: cache.select(packed, q, sel), lambda: cache.attend(packed, q[:, :250], sel, out),
+              lambda: cache.append(packed, q[:, :128], q[:, 128:]), lambda: cache.attend(packed, q.cpu(), sel, out)):
+        with pytest.raises(ResidentError) as e:
+            f()
+        assert e.value.status == abi.BAD_ARGUMENT
+    torch.cuda.synchronize()
+    assert ops.launch_count() == before and out.eq(5).all()
+    cache.attend(packed, q, sel, out)
+    torch.cuda.synchronize()
+    assert ops.launch_count() == before + 1 and torch.cuda.current_device() == device and out.eq(0).all()
 
 
 class Step:
