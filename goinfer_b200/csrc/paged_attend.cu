@@ -46,18 +46,22 @@ __device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned&
     lo = *reinterpret_cast<const unsigned*>(&l);
 }
 
+// A part's weight in the whole: f over the sum l; 0 where no key was seen, NaN where l is.
+__device__ __forceinline__ float whole(float f, float l) { return l > 0.f || l != l ? f / l : 0.f; }
+
 template <int HD>
 struct AttendShape {
     static constexpr int KS = HD / 16, CPR = HD / 8, ROWB = HD * 2, TILE = 16 * ROWB, CPL = 16 * CPR / 32;
     static constexpr size_t ring = (size_t)kAttWarps * kAttStages * 2 * TILE;
-    // what the cluster's CTAs send this one: its share of the outputs of each, then their maxima and sums
-    static constexpr size_t inbox = 8 * HD + 2 * kAttMaxCluster * 8;
+    static constexpr size_t inbox = 8 * HD + 32 * (kAttMaxCluster - 1);  // what the CTAs send this one: of each, this one's share
     static constexpr size_t smem(int n_select) { return ring + sizeof(float) * inbox + sizeof(int2) * (size_t)n_select; }
     static constexpr int ACC = HD + 4;  // floats between heads in the warps' states: the fragments' stores meet no bank twice
 };
 
+// Two CTAs an SM at least: with all the registers that leaves it the compiler keeps more of a tile's steps in flight than it would
+// by itself (4 x 131k keys 45.4 against 49.6 us).
 template <int HD>
-__global__ void __launch_bounds__(kAttThreads) paged_attend_kernel(const b200_paged_cache c, const int32_t* __restrict__ row_slot,
+__global__ void __launch_bounds__(kAttThreads, 2) paged_attend_kernel(const b200_paged_cache c, const int32_t* __restrict__ row_slot,
                                                                    const int32_t* __restrict__ row_pos, const float* __restrict__ q, size_t ldq, int G,
                                                                    float scale, float cap, const int32_t* __restrict__ sel, int n_select,
                                                                    float* __restrict__ out, size_t ldo) {
@@ -68,6 +72,8 @@ __global__ void __launch_bounds__(kAttThreads) paged_attend_kernel(const b200_pa
     float* inbox = reinterpret_cast<float*>(att_smem + S::ring);
     int2* list = reinterpret_cast<int2*>(inbox + S::inbox);
     __shared__ int s_count[kAttWarps];
+    __shared__ float s_max[kAttWarps][8], s_sum[kAttWarps][8], s_factor[kAttMaxCluster][8];  // [][head]
+    __shared__ float in_max[kAttMaxCluster][8], in_sum[kAttMaxCluster][8];                   // of the cluster's CTAs
     const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
     const int r = blockIdx.x / ctas, kvh = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
@@ -241,13 +247,11 @@ __global__ void __launch_bounds__(kAttThreads) paged_attend_kernel(const b200_pa
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     pdl_trigger();  // not before: CTAs of the next kernel beside this one's would lie unevenly (ragged lists 15.0 against 13.3 us)
     __syncthreads();
-    // join the warps (in the rings' room): acc[warp][head][dim], then maximum and sum [warp][head]
+    // join the warps (in the rings' room): acc[warp][head][dim]; maximum and sum [warp][head] become the warps' factors
     float* acc = reinterpret_cast<float*>(att_smem);
-    float* sm_m = acc + kAttWarps * 8 * S::ACC;
-    float* sm_l = sm_m + kAttWarps * 8;
-    if (tig == 0 && gid < G) {
-        sm_m[warp * 8 + gid] = m_run;
-        sm_l[warp * 8 + gid] = l_run;
+    if (tig == 0) {
+        s_max[warp][gid] = m_run;
+        s_sum[warp][gid] = l_run;
     }
 #pragma unroll
     for (int mt = 0; mt < KS; mt++) {
@@ -255,54 +259,60 @@ __global__ void __launch_bounds__(kAttThreads) paged_attend_kernel(const b200_pa
         if (h0 < G) { acc[(warp * 8 + h0) * S::ACC + d0] = o[mt][0]; acc[(warp * 8 + h0) * S::ACC + d0 + 8] = o[mt][2]; }
         if (h1 < G) { acc[(warp * 8 + h1) * S::ACC + d0] = o[mt][1]; acc[(warp * 8 + h1) * S::ACC + d0 + 8] = o[mt][3]; }
     }
-    __syncthreads();
     if (ctas > 1) cluster_wait();  // the CTAs have started: their shared memory may be written
-    // value idx of the CTA's state goes to the CTA that owns it (share = values a CTA owns), maxima and sums to all
-    const int values = G * HD, share = values / ctas;
+    __syncthreads();
+    float M = -INFINITY, l = 0.f;
+    if (warp == 0) {  // a lane: warp lane / 8, head gid of lane % 8
+        const int w = lane >> 3, g = lane & 7;
+#pragma unroll
+        for (int i = 0; i < kAttWarps; i++) M = fmaxf(M, s_max[i][g]);
+        const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int i = 0; i < kAttWarps; i++) l = fmaf(s_sum[i][g], __expf(s_max[i][g] - ref), l);
+        const float f = __expf(s_max[w][g] - ref);
+        s_factor[w][g] = ctas > 1 ? f : whole(f, l);
+        for (int to = w; ctas > 1 && to < ctas; to += 4) {
+            cluster_store(cluster_addr(&in_max[rank][g], to), M);
+            cluster_store(cluster_addr(&in_sum[rank][g], to), l);
+        }
+    }
+    __syncthreads();
+    // Value idx of the CTA's state (head, dim) belongs to CTA (idx / 32) % ctas, where it is number idx / 32 / ctas * 32 + idx % 32:
+    // what a warp sends goes to one CTA.
+    const int values = G * HD, log_ctas = 31 - __clz(ctas), share = ((values >> 5) + ctas - 1) >> log_ctas << 5;
     float* out_row = out + (size_t)r * ldo + (size_t)kvh * values;
     for (int idx = tid; idx < values; idx += kAttThreads) {
         const int g = idx / HD, e = idx % HD;
-        float M = -INFINITY;
+        float tot = 0.f;
 #pragma unroll
-        for (int w = 0; w < kAttWarps; w++) M = fmaxf(M, sm_m[w * 8 + g]);
-        const float ref = M == -INFINITY ? 0.f : M;
-        float tot = 0.f, l = 0.f;
-#pragma unroll
-        for (int w = 0; w < kAttWarps; w++) {
-            const float f = __expf(sm_m[w * 8 + g] - ref);
-            tot = fmaf(acc[(w * 8 + g) * S::ACC + e], f, tot);
-            l = fmaf(sm_l[w * 8 + g], f, l);
-        }
-        if (ctas == 1) {
-            out_row[idx] = l > 0.f || l != l ? tot / l : 0.f;
-        } else {
-            cluster_store(cluster_addr(inbox + rank * share + idx % share, idx / share), tot);
-            if (e < ctas) {
-                cluster_store(cluster_addr(inbox + 8 * HD + rank * 8 + g, e), M);
-                cluster_store(cluster_addr(inbox + 8 * HD + (kAttMaxCluster + rank) * 8 + g, e), l);
-            }
-        }
+        for (int w = 0; w < kAttWarps; w++) tot = fmaf(acc[(w * 8 + g) * S::ACC + e], s_factor[w][g], tot);
+        if (ctas == 1) out_row[idx] = tot;
+        else cluster_store(cluster_addr(inbox + rank * share + ((idx >> (5 + log_ctas)) << 5 | (idx & 31)), (idx >> 5) & (ctas - 1)), tot);
     }
     if (ctas == 1) return;
     cluster_sync();  // what the CTAs sent has arrived
+    if (tid < 8 * kAttMaxCluster) {
+        const int w = tid >> 3, g = tid & 7;
+        M = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < kAttMaxCluster; i++)
+            if (i < ctas) M = fmaxf(M, in_max[i][g]);
+        const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int i = 0; i < kAttMaxCluster; i++)
+            if (i < ctas) l = fmaf(in_sum[i][g], __expf(in_max[i][g] - ref), l);
+        if (w < ctas) s_factor[w][g] = whole(__expf(in_max[w][g] - ref), l);
+    }
+    __syncthreads();
     for (int i = tid; i < share; i += kAttThreads) {
-        const int idx = rank * share + i, g = idx / HD;
-        const float* ms = inbox + 8 * HD + g;
-        float M = -INFINITY;
+        const int idx = ((i >> 5 << log_ctas) + rank) << 5 | (i & 31), g = idx / HD;
+        if (idx >= values) break;
+        float tot = 0.f;
 #pragma unroll
         for (int w = 0; w < kAttMaxCluster; w++)
-            if (w < ctas) M = fmaxf(M, ms[w * 8]);
-        const float ref = M == -INFINITY ? 0.f : M;
-        float tot = 0.f, l = 0.f;
-#pragma unroll
-        for (int w = 0; w < kAttMaxCluster; w++) {
-            if (w < ctas) {
-                const float f = __expf(ms[w * 8] - ref);
-                tot = fmaf(inbox[w * share + i], f, tot);
-                l = fmaf(ms[(kAttMaxCluster + w) * 8], f, l);
-            }
-        }
-        out_row[idx] = l > 0.f || l != l ? tot / l : 0.f;
+            if (w < ctas) tot = fmaf(inbox[w * share + i], s_factor[w][g], tot);
+        out_row[idx] = tot;
     }
 }
 
