@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(32 * kAppendMaxWarps) paged_append_kernel(cons
                                                                             size_t ldv, int rows_per_cta, int parts) {
     pdl_trigger();
     pdl_wait();
-    constexpr int LPR = HD / 4, RPW = 32 / LPR, U = 4;  // lanes a row, rows a warp at a time, loads in flight
+    constexpr int LPR = HD / 4, RPW = 32 / LPR, U = 4, OLD = 16;  // lanes a row, rows a warp at a time, loads in flight of new and of older rows
     __shared__ Bounds4 joined[kAppendMaxWarps][LPR];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, br = c.block_rows;
     const int sub = lane % LPR, row_of = lane / LPR;
@@ -289,13 +289,13 @@ __global__ void __launch_bounds__(32 * kAppendMaxWarps) paged_append_kernel(cons
             }
             if (!c.key_bounds) continue;
             const int o0 = first * part / parts, o1 = first * (part + 1) / parts;
-            for (int j = o0 + row_of; j < o1; j += U * RPW) {
-                uint2 old[U];
+            for (int j = o0 + row_of; j < o1; j += OLD * RPW) {
+                uint2 old[OLD];
 #pragma unroll
-                for (int i = 0; i < U; i++)
+                for (int i = 0; i < OLD; i++)
                     if (j + i * RPW < o1) old[i] = kt[(size_t)(j + i * RPW) * LPR];
 #pragma unroll
-                for (int i = 0; i < U; i++)
+                for (int i = 0; i < OLD; i++)
                     if (j + i * RPW < o1) bounds.fold(old[i], old[i]);
             }
             if constexpr (RPW == 2) {
@@ -399,12 +399,14 @@ extern "C" int b200_paged_append(b200_ctx* ctx, const b200_paged_cache* c, const
     if (ctx->device < 0) B200_FAIL(ctx, B200_CUDA_ERROR, "b200_paged_append: the context has no device");
     DeviceScope dev;
     CUDA_TRY(ctx, dev.enter(ctx->device));
-    // Few rows are decode steps: a CTA looks at one, and with tall blocks sixteen warps share the older rows to be read. Many rows
-    // are prompts, whose runs fill blocks: a CTA that finds no run among its rows costs about as much as 4 ns of the GPU, so it
-    // looks at more (32768 rows of 8 heads of 128 in blocks of 64: 139, 82, 74, 68 us with 1, 4, 8, 32 rows a CTA; 2115 rows in
-    // seven chunks with blocks of 32: 8.1, 5.3, 5.5, 7.2 us).
-    const int rows = r->n_rows > 32 * ctx->sm_count ? 32 : r->n_rows > 4 * ctx->sm_count ? 4 : 1;
-    const int warps = rows > 1 || c->block_rows < 32 ? 8 : kAppendMaxWarps;
+    // Few rows are decode steps: a CTA looks at one, and while there is an SM for each, with tall blocks sixteen warps share the
+    // older rows to be read. Many rows are prompts, whose runs fill blocks: a CTA that finds no run among its rows costs about
+    // as much as 4 ns of the GPU, so it looks at more, as long as four CTAs an SM are left (32768 rows of 8 heads of 128 in
+    // blocks of 64: 139, 82, 74, 68 us with 1, 4, 8, 32 rows a CTA; 2115 rows in seven chunks with blocks of 32: 8.1, 5.3, 5.5,
+    // 7.2 us; 5529 rows of one head of 64 in 291 chunks: 6.9 us with 16, 8.4 with 32).
+    int rows = 1;
+    while (rows < 32 && r->n_rows > 4 * ctx->sm_count * rows) rows *= 2;
+    const int warps = r->n_rows <= ctx->sm_count && c->block_rows >= 32 ? kAppendMaxWarps : 8;
     const int parts = c->n_kv_heads < warps ? warps / c->n_kv_heads : 1;
     const int threads = 32 * (c->n_kv_heads < warps ? c->n_kv_heads * parts : warps);
     auto kernel = c->head_dim == 128 ? paged_append_kernel<128> : paged_append_kernel<64>;
