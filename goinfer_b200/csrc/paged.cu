@@ -209,16 +209,6 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const PlanArgs 
 // head's rows and join their bounds in shared memory.
 constexpr int kAppendMaxWarps = 16;
 
-__device__ __forceinline__ unsigned min_nan2(unsigned a, unsigned b) {
-    unsigned r;
-    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ unsigned max_nan2(unsigned a, unsigned b) {
-    unsigned r;
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 struct Bounds4 {  // of four dims
     uint2 lo = {0x7c007c00u, 0x7c007c00u}, hi = {0xfc00fc00u, 0xfc00fc00u};  // +inf, -inf
     __device__ __forceinline__ void fold(uint2 l, uint2 h) {

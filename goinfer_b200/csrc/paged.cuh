@@ -77,6 +77,18 @@ inline void launch_cluster(void (*kernel)(KArgs...), int cluster, dim3 grid, dim
     cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);  // an error surfaces in LAUNCH_CHECK's cudaGetLastError
 }
 
+// pairs of halves; a NaN on either side stays
+__device__ __forceinline__ unsigned min_nan2(unsigned a, unsigned b) {
+    unsigned r;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned max_nan2(unsigned a, unsigned b) {
+    unsigned r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));

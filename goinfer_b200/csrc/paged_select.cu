@@ -13,7 +13,7 @@
 // q scaled by a power of two (largest |q| in [1, 2)) and split into fp16 parts hi + 2^-11 lo, products exact, fp32 sums. The
 // split leaves at most 2^-22 |q_d| or 2^-36; a step that adds 16 products to the sum is off by at most 17 * 2^-23 of the terms'
 // absolute sum S, 16 of them by 2^-14.9 S. E = 2^-13 S + 2^-12 covers it (128 dims of the largest fp16 bound times 2^-36 are
-// 2^-13), with S from the absolute values of the same operands. The true m-th score lies within E of the m-th s~, so a block whose s~ is more than
+// 2^-13), with S = sum |q_d| max(|lo_d|, |hi_d|), which is no less than the terms' sum, from the same unit. The true m-th score lies within E of the m-th s~, so a block whose s~ is more than
 // 2E above (below) that is in (out) for certain; only the blocks between (a handful) are scored in f64. An infinity or a
 // NaN anywhere makes E infinite, and every block is scored in f64.
 //
@@ -153,7 +153,7 @@ __device__ __forceinline__ unsigned long long exact_key(const b200_paged_cache& 
 
 // Four CTAs an SM: the 128 registers this leaves a thread hold a run's bounds (64) on their way; with fewer the compiler starts
 // the products before the last load is out (batch 66 us either way, long contexts 50 against 58 us).
-template <int HD>
+template <int HD, bool NARROW>
 __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200_paged_cache c, const int32_t* __restrict__ row_slot,
                                                                    const int32_t* __restrict__ row_pos, const float* __restrict__ q, size_t ldq, int G,
                                                                    int n_first, int n_recent, int n_select, int max_chunk, int32_t* __restrict__ sel) {
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
     unsigned* doubt_bits = in_bits + max_chunk / 32;
     __shared__ __align__(16) unsigned hist[kSelBins];
     __shared__ __align__(16) float sq[8][HD];
-    __shared__ __align__(16) uint4 q_frag[HD / 32][4][32];  // chunk of dims, part (q > 0 hi, lo; q <= 0 hi, lo), lane
+    __shared__ __align__(16) uint4 q_frag[HD / 32][NARROW ? 3 : 5][32];  // chunk of dims, part (q > 0, q <= 0, |q|; their lo), lane
     // what the CTAs tell one another, by rank (and warp)
     __shared__ float s_err[kSelMaxCluster * kSelWarps], s_min[kSelMaxCluster * kSelWarps], s_max[kSelMaxCluster * kSelWarps];
     __shared__ unsigned s_word[kSelMaxCluster * kSelWarps], s_top[kSelMaxCluster * kSelWarps];
@@ -210,8 +210,10 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
     tbl += from;
     {
         // Fragments: row of A = block, column of B = head. A lane's words of a 16-byte chunk are taken as the dims of its
-        // places in the k steps; q is laid out by the same rule, so a bound is loaded as it lies.
+        // places in the k steps; q is laid out by the same rule, so a bound is loaded as it lies. With up to four heads (NARROW)
+        // columns 0 .. 3 hold the parts hi of q and 4 .. 7 the parts lo, else lo takes products of its own.
         constexpr int CH = HD / 32;  // 16-byte chunks of a row per lane: chunks tig, tig + 4, ...
+        constexpr unsigned abs2 = 0x7fff7fffu;
         const int gid = lane >> 2, tig = lane & 3;
         int b0 = 16 * warp;
         auto page_of = [&](int b) { return b < own ? tbl[b] : 0; };
@@ -222,7 +224,8 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
         // the columns' powers of two against the group's largest; columns past the group repeat its first head
         float f0, f1;
         {
-            const float* qp = sq[gid < G ? gid : 0] + 8 * tig;
+            const int head = NARROW ? gid & 3 : gid;
+            const float* qp = sq[head < G ? head : 0] + 8 * tig;
             float most = 0.f;
 #pragma unroll
             for (int i = 0; i < 2 * CH; i++) {
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) e_max = max(e_max, __shfl_xor_sync(0xffffffffu, e_max, o));
             const float f = pow2(max(-126, e - e_max));
-            f0 = __shfl_sync(0xffffffffu, f, 8 * tig);
+            f0 = __shfl_sync(0xffffffffu, f, 8 * tig);  // of column 2 tig: that column's lanes hold its head's factor
             f1 = __shfl_sync(0xffffffffu, f, 8 * tig + 4);
             auto split = [](float a, float b, unsigned& hi, unsigned& lo) {
                 hi = half2_bits(a, b);
@@ -248,16 +251,21 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
             if (warp < CH) {  // each warp lays out one chunk of the dims; word j of a part: dims 2j, 2j + 1 of the lane's eight
                 const float4 u = *reinterpret_cast<const float4*>(qp + 32 * warp), v = *reinterpret_cast<const float4*>(qp + 32 * warp + 4);
                 const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-                unsigned w[4][4];
+                unsigned w[5][4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const float a = x[2 * j] * down0 * down1, b = x[2 * j + 1] * down0 * down1;
                     // !(q > 0) goes with the lower bounds, a NaN as well
-                    split(a > 0.f ? a : 0.f, b > 0.f ? b : 0.f, w[0][j], w[1][j]);
-                    split(a > 0.f ? 0.f : a, b > 0.f ? 0.f : b, w[2][j], w[3][j]);
+                    split(a > 0.f ? a : 0.f, b > 0.f ? b : 0.f, w[0][j], w[3][j]);
+                    split(a > 0.f ? 0.f : a, b > 0.f ? 0.f : b, w[1][j], w[4][j]);
+                    w[2][j] = w[0][j] | (w[1][j] & abs2);
+                    if (NARROW && gid >= 4) {
+                        w[0][j] = w[3][j];
+                        w[1][j] = w[4][j];
+                    }
                 }
 #pragma unroll
-                for (int t = 0; t < 4; t++) q_frag[warp][t][lane] = make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]);
+                for (int t = 0; t < (NARROW ? 3 : 5); t++) q_frag[warp][t][lane] = make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]);
             }
         }
         __syncthreads();
@@ -281,31 +289,43 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
             }
             page0 = page_of(b0 + kSelRun + gid);
             page1 = page_of(b0 + kSelRun + 8 + gid);
-            float hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0}, up[4] = {0, 0, 0, 0}, dn[4] = {0, 0, 0, 0};
-            constexpr unsigned abs2 = 0x7fff7fffu;
+            float up[4] = {0, 0, 0, 0}, dn[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0}, sum[4] = {0, 0, 0, 0};
             // two k steps on a chunk of the bounds: words 0, 1 and words 2, 3
-            auto chunk = [&](const uint4& a, const uint4& b, const uint4& qh, const uint4& ql, float (&sum)[4]) {
-                mma16816(hi, a.x, b.x, a.y, b.y, qh.x, qh.y);
-                mma16816(lo, a.x, b.x, a.y, b.y, ql.x, ql.y);
-                mma16816(sum, a.x & abs2, b.x & abs2, a.y & abs2, b.y & abs2, qh.x, qh.y);
-                mma16816(hi, a.z, b.z, a.w, b.w, qh.z, qh.w);
-                mma16816(lo, a.z, b.z, a.w, b.w, ql.z, ql.w);
-                mma16816(sum, a.z & abs2, b.z & abs2, a.w & abs2, b.w & abs2, qh.z, qh.w);
+            auto product = [](float (&c)[4], const uint4& a, const uint4& b, const uint4& q) {
+                mma16816(c, a.x, b.x, a.y, b.y, q.x, q.y);
+                mma16816(c, a.z, b.z, a.w, b.w, q.z, q.w);
+            };
+            auto larger = [](const uint4& a, const uint4& b) {  // of the magnitudes; a NaN stays
+                return make_uint4(max_nan2(a.x & abs2, b.x & abs2), max_nan2(a.y & abs2, b.y & abs2), max_nan2(a.z & abs2, b.z & abs2),
+                                  max_nan2(a.w & abs2, b.w & abs2));
             };
 #pragma unroll
             for (int i = 0; i < CH; i++) {
-                chunk(h0[i], h1[i], q_frag[i][0][lane], q_frag[i][1][lane], up);
-                chunk(l0[i], l1[i], q_frag[i][2][lane], q_frag[i][3][lane], dn);
+                product(up, h0[i], h1[i], q_frag[i][0][lane]);
+                product(dn, l0[i], l1[i], q_frag[i][1][lane]);
+                product(sum, larger(h0[i], l0[i]), larger(h1[i], l1[i]), q_frag[i][2][lane]);
+                if constexpr (!NARROW) {
+                    product(lo, h0[i], h1[i], q_frag[i][3][lane]);
+                    product(lo, l0[i], l1[i], q_frag[i][4][lane]);
+                }
             }
             // columns 2 tig and 2 tig + 1 of rows gid (values 0, 1) and gid + 8 (values 2, 3)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const bool ok = h ? ok1 : ok0;
                 const int b = b0 + 8 * h + gid;
-                const float E0 = fmaf(up[2 * h] - dn[2 * h], k0, floor0), E1 = fmaf(up[2 * h + 1] - dn[2 * h + 1], k1, floor1);
-                float s = fmaxf(fmaf(lo[2 * h], 0x1p-11f, hi[2 * h]) * f0, fmaf(lo[2 * h + 1], 0x1p-11f, hi[2 * h + 1]) * f1);
+                const float E0 = fmaf(sum[2 * h], k0, floor0), E1 = fmaf(sum[2 * h + 1], k1, floor1);
+                float hi0 = up[2 * h] + dn[2 * h], hi1 = up[2 * h + 1] + dn[2 * h + 1], lo0 = lo[2 * h], lo1 = lo[2 * h + 1];
+                if constexpr (NARROW) {  // the same head's other part is two lanes away
+                    const float other0 = __shfl_xor_sync(0xffffffffu, hi0, 2), other1 = __shfl_xor_sync(0xffffffffu, hi1, 2);
+                    lo0 = tig < 2 ? other0 : hi0;
+                    lo1 = tig < 2 ? other1 : hi1;
+                    hi0 = tig < 2 ? hi0 : other0;
+                    hi1 = tig < 2 ? hi1 : other1;
+                }
+                float s = fmaxf(fmaf(lo0, 0x1p-11f, hi0) * f0, fmaf(lo1, 0x1p-11f, hi1) * f1);
                 s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 1));
-                s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 2));
+                if constexpr (!NARROW) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 2));
                 if (ok) {
                     err_bits = max(err_bits, max(__float_as_uint(E0) & 0x7fffffffu, __float_as_uint(E1) & 0x7fffffffu));
                     mn = fminf(mn, s);
@@ -559,13 +579,14 @@ extern "C" int b200_paged_select(b200_ctx* ctx, const b200_paged_cache* c, const
     DeviceScope dev;
     CUDA_TRY(ctx, dev.enter(ctx->device));
     const int G = n_heads / c->n_kv_heads;
-    auto kernel = c->head_dim == 128 ? paged_select_kernel<128> : paged_select_kernel<64>;
-    static SmemLimit limit[2];
+    auto kernel = c->head_dim == 128 ? (G <= 4 ? paged_select_kernel<128, true> : paged_select_kernel<128, false>)
+                                     : (G <= 4 ? paged_select_kernel<64, true> : paged_select_kernel<64, false>);
+    static SmemLimit limit[4];
     int ctas = 1;
     while (ctas < kSelMaxCluster && (long long)r->n_rows * c->n_kv_heads * ctas < 2 * ctx->sm_count && c->max_blocks > kSelRun * ctas) ctas *= 2;
     const int chunk = ceil_div(c->max_blocks, kSelRun * ctas) * kSelRun;  // of one CTA
     auto smem = [](int blocks) { return (size_t)blocks * 4 + 2 * ((size_t)blocks / 8); };
-    CUDA_TRY(ctx, limit[c->head_dim == 128].raise(kernel, ctx->device, smem(kSelMaxBlocks)));
+    CUDA_TRY(ctx, limit[2 * (c->head_dim == 128) + (G <= 4)].raise(kernel, ctx->device, smem(kSelMaxBlocks)));
     launch_cluster(kernel, ctas, dim3((unsigned)(r->n_rows * ctas), c->n_kv_heads), dim3(kSelThreads), smem(chunk), ctx->stream, *c, r->row_slot, r->row_pos, q,
                    (size_t)ldq, G, n_first, n_recent, n_select, chunk, sel);
     LAUNCH_CHECK(ctx);
