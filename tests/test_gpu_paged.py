@@ -665,3 +665,28 @@ def test_a_full_list_gives_dense_attention(ops):
     torch.cuda.synchronize()
     x = (q.reshape(rows, kv, G, hd).abs().amax() * hd * k_pool.abs().amax().float() * hd ** -0.5).item()
     _close(out, dense.double(), min(x, math.sqrt(hd) * 1.0))
+
+
+def test_the_documented_step_runs():
+    """The step of the integration guide, as it stands there, over two steps of eight sequences."""
+    import os
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")).read()
+    code = text[text.index("import torch\nfrom goinfer_b200.ops import Ops\nfrom goinfer_b200.paged"):]
+    setup, step = code[:code.index("```")].split("layers[0].plan", 1)
+    env = {}
+    exec(setup, env)
+    length = torch.zeros(8, dtype=torch.int32, device="cuda")
+    for new in ([5, 0, 17, 1, 2, 3, 4, 8], [1, 1, 1, 1, 1, 1, 1, 1]):
+        env.update(kv_len=length, n_new=dev(new), k=torch.randn(64, 8, 128, device="cuda"), v=torch.randn(64, 8, 128, device="cuda"),
+                   q=torch.randn(64, 32, 128, device="cuda"))
+        exec("layers[0].plan" + step, env)
+        torch.cuda.synchronize()
+        assert env["rows"].status.tolist()[:2] == [0, sum(new)]
+        length = length + dev(new)
+    # a sequence's second step sees what the first stored, in both layers' pools
+    r, cache = 2, env["layers"][1]
+    keys = cache._keep[4][env["table"][2, :2].long()].transpose(1, 2).reshape(32, 8, 128)[:18]
+    values = cache._keep[5][env["table"][2, :2].long()].transpose(1, 2).reshape(32, 8, 128)[:18]
+    x = torch.einsum("hgd,khd->hgk", env["q"][r].double().reshape(8, 4, 128), keys.double()) * 128 ** -0.5
+    want = torch.einsum("hgk,khd->hgd", torch.softmax(x, -1), values.double()).reshape(32, 128)
+    _close(env["out"][r], want, torch.einsum("hgd,khd->hgk", env["q"][r].double().reshape(8, 4, 128).abs(), keys.double().abs()).max().item() * 128 ** -0.5)
