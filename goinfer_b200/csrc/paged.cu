@@ -223,8 +223,8 @@ __device__ __forceinline__ uint2 to_half4(float4 x) {
 
 // rows_per_cta: packed rows whose runs a CTA looks for; parts: warps that share a head (when above 1, the CTA has heads * parts warps)
 template <int HD>
-__global__ void __launch_bounds__(32 * kAppendMaxWarps) paged_append_kernel(const b200_paged_cache c, const int32_t* __restrict__ slot_map, int n_rows,
-                                                                            const float* __restrict__ k, size_t ldk, const float* __restrict__ v,
+__global__ void __launch_bounds__(32 * kAppendMaxWarps) paged_append_kernel(const b200_paged_cache c, const int32_t* slot_map, int n_rows,
+                                                                            const float* k, size_t ldk, const float* v,
                                                                             size_t ldv, int rows_per_cta, int parts) {
     pdl_trigger();
     pdl_wait();

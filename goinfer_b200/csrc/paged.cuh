@@ -53,7 +53,9 @@ struct SmemLimit {
 
 #ifdef __CUDACC__
 // launch_pdl (common.cuh: its rule holds here too) with clusters of `cluster` CTAs along x. Every kernel over the paged cache
-// goes through one of the two and waits before it reads anything, so that the launches of a step's calls overlap.
+// goes through one of the two and waits before it reads anything, so that the launches of a step's calls overlap. What it
+// reads may have been written while it was already resident, so its pointers are not __restrict__: the compiler would turn
+// their loads into non-coherent ones, which ask for memory that nobody writes during the kernel.
 template <typename... KArgs, typename... Args>
 inline void launch_cluster(void (*kernel)(KArgs...), int cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
     cudaLaunchConfig_t cfg = {};

@@ -61,10 +61,10 @@ struct AttendShape {
 // Two CTAs an SM at least: with all the registers that leaves it the compiler keeps more of a tile's steps in flight than it would
 // by itself (4 x 131k keys 45.4 against 49.6 us).
 template <int HD>
-__global__ void __launch_bounds__(kAttThreads, 2) paged_attend_kernel(const b200_paged_cache c, const int32_t* __restrict__ row_slot,
-                                                                   const int32_t* __restrict__ row_pos, const float* __restrict__ q, size_t ldq, int G,
-                                                                   float scale, float cap, const int32_t* __restrict__ sel, int n_select,
-                                                                   float* __restrict__ out, size_t ldo) {
+__global__ void __launch_bounds__(kAttThreads, 2) paged_attend_kernel(const b200_paged_cache c, const int32_t* row_slot,
+                                                                   const int32_t* row_pos, const float* q, size_t ldq, int G,
+                                                                   float scale, float cap, const int32_t* sel, int n_select,
+                                                                   float* out, size_t ldo) {
     pdl_wait();
     using S = AttendShape<HD>;
     constexpr int KS = S::KS, CPR = S::CPR, ROWB = S::ROWB, TILE = S::TILE, CPL = S::CPL;

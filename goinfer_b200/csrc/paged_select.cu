@@ -13,9 +13,10 @@
 // q scaled by a power of two (largest |q| in [1, 2)) and split into fp16 parts hi + 2^-11 lo, products exact, fp32 sums. The
 // split leaves at most 2^-22 |q_d| or 2^-36; a step that adds 16 products to the sum is off by at most 17 * 2^-23 of the terms'
 // absolute sum S, 16 of them by 2^-14.9 S. E = 2^-13 S + 2^-12 covers it (128 dims of the largest fp16 bound times 2^-36 are
-// 2^-13), with S = sum |q_d| max(|lo_d|, |hi_d|), which is no less than the terms' sum, from the same unit. The true m-th score lies within E of the m-th s~, so a block whose s~ is more than
-// 2E above (below) that is in (out) for certain; only the blocks between (a handful) are scored in f64. An infinity or a
-// NaN anywhere makes E infinite, and every block is scored in f64.
+// 2^-13), with S = sum |q_d| max(|lo_d|, |hi_d|), which is no less than the terms' sum, from the same unit. The true m-th
+// score lies within E of the m-th s~, so a block whose s~ is more than 2E above (below) that is in (out) for certain; only
+// the blocks between (a handful) are scored in f64. An infinity or a NaN anywhere makes E infinite, and every block is
+// scored in f64.
 //
 // One cluster of CTAs per (row, kv head). Each CTA scores a run of the blocks, keeps its s~ in shared memory and decides about
 // its own blocks; what the cluster has to agree on goes through distributed shared memory, every CTA reading the same: the
@@ -29,7 +30,7 @@ namespace {
 constexpr int kSelThreads = 128, kSelWarps = kSelThreads / 32;
 constexpr int kSelMaxBlocks = 24576;  // a CTA that is alone holds a score and two bits for each in shared memory
 constexpr int kSelMaxList = 2048;
-constexpr int kSelBins = 512;        // four a thread
+constexpr int kSelBins = 512;         // four a thread
 constexpr int kSelDoubt = 256;        // blocks in doubt that are ranked in a list; more are selected among in place
 constexpr int kSelMaxCluster = 8;
 constexpr int kSelRun = 16 * kSelWarps;  // blocks a CTA scores at a time
@@ -42,7 +43,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1
 // A load that stays where it is written: all of a run's loads go out before its first product waits for one.
 __device__ __forceinline__ uint4 load16(const uint8_t* p) {
     uint4 v;
-    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }  // -126 <= e <= 127
@@ -154,9 +155,9 @@ __device__ __forceinline__ unsigned long long exact_key(const b200_paged_cache& 
 // Four CTAs an SM: the 128 registers this leaves a thread hold a run's bounds (64) on their way; with fewer the compiler starts
 // the products before the last load is out (batch 66 us either way, long contexts 50 against 58 us).
 template <int HD, bool NARROW>
-__global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200_paged_cache c, const int32_t* __restrict__ row_slot,
-                                                                   const int32_t* __restrict__ row_pos, const float* __restrict__ q, size_t ldq, int G,
-                                                                   int n_first, int n_recent, int n_select, int max_chunk, int32_t* __restrict__ sel) {
+__global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200_paged_cache c, const int32_t* row_slot,
+                                                                   const int32_t* row_pos, const float* q, size_t ldq, int G,
+                                                                   int n_first, int n_recent, int n_select, int max_chunk, int32_t* sel) {
     pdl_wait();
     // the CTA's blocks: s~ (with many blocks in doubt, words of their keys), a bit for those that are in, one for those in doubt
     extern __shared__ __align__(16) float sel_score[];

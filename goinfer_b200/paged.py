@@ -119,7 +119,7 @@ class PagedCache:
                                 None if key_bounds is None else _array("key_bounds", key_bounds, f16, (n_blocks, kv, 2, hd), dev), table,
                                 _array("seq_blocks", seq_blocks, i32, (self.n_seqs,), dev), _array("free_blocks", free_blocks, i32, (n_blocks,), dev),
                                 _array("free_count", free_count, i32, (1,), dev), n_blocks, self.n_seqs, max_blocks, block_rows, kv, hd)
-        self._c, self._ctx = C.addressof(self.c), ops.ctx.value
+        self._c, self._drv = C.addressof(self.c), ops.drv
         lib = ops.lib
         vp, i, f = C.c_void_p, C.c_int, C.c_float
         for fn, types in ((lib.b200_paged_plan, (vp, vp, vp, vp, vp)), (lib.b200_paged_append, (vp, vp, vp, vp, i, vp, i)),
@@ -146,7 +146,7 @@ class PagedCache:
         if rows.n_seqs != self.n_seqs:
             _refuse(f"rows are for {rows.n_seqs} sequences, the cache has {self.n_seqs}")
         shape, device = (self.n_seqs,), self.device
-        st = self._plan(self._ctx, self._c, rows._c, _array("kv_len", kv_len, _I32, shape, device), _array("n_new", n_new, _I32, shape, device))
+        st = self._plan(self._drv.ctx.value, self._c, rows._c, _array("kv_len", kv_len, _I32, shape, device), _array("n_new", n_new, _I32, shape, device))
         if st:
             self._raise(st)
 
@@ -156,7 +156,7 @@ class PagedCache:
         pv, ldv, wv = _packed("v", v, n, device)
         if wk != self.n_kv_heads * self.head_dim or wv != wk:
             _refuse(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have {self.n_kv_heads} heads of {self.head_dim} a row")
-        st = self._append(self._ctx, self._c, rows._c, pk, ldk, pv, ldv)
+        st = self._append(self._drv.ctx.value, self._c, rows._c, pk, ldk, pv, ldv)
         if st:
             self._raise(st)
 
@@ -165,7 +165,7 @@ class PagedCache:
         pq, ldq, width = _packed("q", q, n, device)
         n_select = sel.shape[-1]
         ps = _array("sel", sel, _I32, (n, self.n_kv_heads, n_select), device)
-        st = self._select(self._ctx, self._c, rows._c, pq, ldq, self._heads("q", width), n_first, n_recent, n_select, ps)
+        st = self._select(self._drv.ctx.value, self._c, rows._c, pq, ldq, self._heads("q", width), n_first, n_recent, n_select, ps)
         if st:
             self._raise(st)
 
@@ -177,6 +177,6 @@ class PagedCache:
             _refuse(f"out has shape {tuple(out.shape)}, q {tuple(q.shape)}")
         n_select = sel.shape[-1]
         ps = _array("sel", sel, _I32, (n, self.n_kv_heads, n_select), device)
-        st = self._attend(self._ctx, self._c, rows._c, pq, ldq, self._heads("q", width), scale, softcap, ps, n_select, po, ldo)
+        st = self._attend(self._drv.ctx.value, self._c, rows._c, pq, ldq, self._heads("q", width), scale, softcap, ps, n_select, po, ldo)
         if st:
             self._raise(st)
