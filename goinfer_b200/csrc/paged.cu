@@ -63,7 +63,7 @@ __device__ __forceinline__ Sums warp_inclusive(Sums v, int lane) {
     return v;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs a, int write_rows) {
+__global__ void __launch_bounds__(kPlanThreads, 1) paged_plan_kernel(const PlanArgs a, int write_rows) {
     pdl_trigger();
     pdl_wait();
     extern __shared__ int plan_smem[];
@@ -72,12 +72,12 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
     int* shrink0 = grow0 + a.n_seqs + 1;      // [n + 1] scan of blocks given back
     __shared__ Sums warp_sum[32];
     __shared__ int first_bad;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n_seqs, br = a.block_rows;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, n = a.n_seqs, br = a.block_rows;
     if (tid == 0) first_bad = n;
     __syncthreads();
 
     // every thread takes a run of sequences; with more than one it looks at them again for the scan
-    const int per = (n + kPlanThreads - 1) / kPlanThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
+    const int per = (n + threads - 1) / threads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
     const int free0 = *a.count;
     int add = 0, want = 0, have = 0;
     auto look = [&](int i) {
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
     if (lane == 31) warp_sum[warp] = scan;
     __syncthreads();
     if (warp == 0) {
-        const Sums t = warp_inclusive(warp_sum[lane], lane);
+        const Sums t = warp_inclusive(32 * lane < threads ? warp_sum[lane] : Sums{0, 0, 0}, lane);
         warp_sum[lane] = t;
     }
     __syncthreads();
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
     const bool bad = bad_seq < n || total.rows > a.n_rows || free0 < 0 || (long long)free0 + S > a.n_blocks;
     const bool full = !bad && G > free0 + S;
     const int rank = (int)cluster_rank(), ctas = (int)cluster_size();
-    const int gtid = rank * kPlanThreads + tid, step = ctas * kPlanThreads;
+    const int gtid = rank * threads + tid, step = ctas * threads;
     auto everyone = [&] {
         if (ctas > 1) cluster_sync(); else __syncthreads();
     };
@@ -365,7 +365,9 @@ extern "C" int b200_paged_plan(b200_ctx* ctx, const b200_paged_cache* c, const b
     // sequences and blocks enough for four a thread: a cluster (2000 sequences with 64000 rows, both calls of a round: 17.3 against
     // 21.8 us with one CTA)
     const int ctas = c->n_seqs + r->n_rows / c->block_rows > 4 * kPlanThreads ? 8 : 1;
-    launch_cluster(paged_plan_kernel, ctas, dim3(ctas), dim3(kPlanThreads), 3 * scan, ctx->stream, a, apart ? 0 : 1);
+    // a decode step's lengths do with eight warps, whose barriers are the cheaper (64 sequences: 6.1 against 6.7 us for two calls)
+    const int threads = c->n_seqs <= 256 && r->n_rows <= 512 ? 256 : kPlanThreads;
+    launch_cluster(paged_plan_kernel, ctas, dim3(ctas), dim3(threads), 3 * scan, ctx->stream, a, apart ? 0 : 1);
     if (apart) {
         LAUNCH_CHECK(ctx);
         CUDA_TRY(ctx, rows_limit.raise(paged_rows_kernel, ctx->device, sizeof(int) * (kPlanMaxSeqs + 1)));
