@@ -22,7 +22,8 @@
 // its own blocks; what the cluster has to agree on goes through distributed shared memory, every CTA reading the same: the
 // range of s~ and E, a histogram in 512 bins that finds the bin of the m-th (taken again inside the bin where that is much
 // wider than E), and the f64 scores of the blocks in doubt. A bit per block says which are in; an ordered pass over the
-// words of bits writes the list.
+// words of bits writes the list. Where the scores are few enough for one CTA, the first one gathers them and does all of
+// that alone.
 #include "paged.cuh"
 
 namespace {
@@ -33,6 +34,7 @@ constexpr int kSelMaxList = 2048;
 constexpr int kSelBins = 512;         // four a thread
 constexpr int kSelDoubt = 256;        // blocks in doubt that are ranked in a list; more are selected among in place
 constexpr int kSelMaxCluster = 8;
+constexpr int kSelGather = 512;       // room for as many scores costs a CTA little, and the choice among them is quick
 constexpr int kSelRun = 16 * kSelWarps;  // blocks a CTA scores at a time
 
 __device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
     __shared__ __align__(16) float sq[8][HD];
     __shared__ __align__(16) uint4 q_frag[HD / 32][NARROW ? 3 : 5][32];  // chunk of dims, part (q > 0, q <= 0, |q|; their lo), lane
     // what the CTAs tell one another, by rank (and warp)
-    __shared__ float s_err[kSelMaxCluster * kSelWarps], s_min[kSelMaxCluster * kSelWarps], s_max[kSelMaxCluster * kSelWarps];
+    __shared__ __align__(16) float s_err[kSelMaxCluster * kSelWarps], s_min[kSelMaxCluster * kSelWarps], s_max[kSelMaxCluster * kSelWarps];
     __shared__ unsigned s_word[kSelMaxCluster * kSelWarps], s_top[kSelMaxCluster * kSelWarps];
     __shared__ int n_in[kSelMaxCluster], n_doubt_of[kSelMaxCluster], n_left[kSelMaxCluster], n_taken[kSelMaxCluster];
     __shared__ unsigned long long doubt_key[kSelDoubt];  // the cluster's blocks in doubt: score and block
@@ -175,7 +177,8 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
     __shared__ int own_doubt[kSelDoubt];
     __shared__ int red_i[kSelWarps];
     __shared__ int s_bin, s_above, s_in, s_doubt;
-    const int ctas = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int ctas = (int)cluster_size();
+    const int rank = (int)cluster_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = blockIdx.x / ctas, kvh = blockIdx.y;
     const int slot = row_slot[r], pos = row_pos[r];
     const float* qr = q + (size_t)r * ldq + (size_t)kvh * G * HD;
@@ -207,8 +210,11 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
     };
     if (ctas > 1) cluster_arrive();
     // this CTA's blocks: from .. from + own - 1 of the middle, 16 a warp at a time
-    const int chunk = (n + kSelRun * ctas - 1) / (kSelRun * ctas) * kSelRun, from = min(n, rank * chunk), own = min(n, from + chunk) - from;
+    const int chunk = (n + kSelRun * ctas - 1) / (kSelRun * ctas) * kSelRun, from = min(n, rank * chunk);
+    int own = min(n, from + chunk) - from;
     tbl += from;
+    // few enough for one CTA: the first one gathers the scores and chooses alone, without another cluster barrier
+    const bool gather = ctas > 1 && n <= max_chunk;
     {
         // Fragments: row of A = block, column of B = head. A lane's words of a 16-byte chunk are taken as the dims of its
         // places in the k steps; q is laid out by the same rule, so a bound is loaded as it lies. With up to four heads (NARROW)
@@ -344,6 +350,11 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
         }
         const float err = __uint_as_float(min(err_bits, 0x7f800000u));
         if (ctas > 1) cluster_wait();  // the CTAs have started: their shared memory may be written
+        if (gather && rank > 0) {
+            __syncthreads();
+            const unsigned there = cluster_addr(sel_score + from, 0);
+            for (int i = 4 * tid; i < own; i += 4 * kSelThreads) cluster_store(there + 4u * (unsigned)i, *reinterpret_cast<const float4*>(sel_score + i));
+        }
         const int at = rank * kSelWarps + warp;
         tell(s_err + at, err);
         tell(s_min + at, mn);
@@ -352,11 +363,18 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
     everyone();
 
     const int told = ctas * kSelWarps;
+    if (gather) {
+        if (rank > 0) return;
+        ctas = 1;
+        own = n;
+    }
     float err = 0.f, lo = INFINITY, hi = -INFINITY;
-    for (int i = 0; i < told; i++) {
-        err = fmaxf(err, s_err[i]);
-        lo = fminf(lo, s_min[i]);
-        hi = fmaxf(hi, s_max[i]);
+    static_assert(kSelWarps == 4, "a CTA's figures are read as one float4");
+    for (int i = 0; i < told; i += 4) {
+        const float4 e = *reinterpret_cast<const float4*>(s_err + i), a = *reinterpret_cast<const float4*>(s_min + i), b = *reinterpret_cast<const float4*>(s_max + i);
+        err = fmaxf(err, fmaxf(fmaxf(e.x, e.y), fmaxf(e.z, e.w)));
+        lo = fminf(lo, fminf(fminf(a.x, a.y), fminf(a.z, a.w)));
+        hi = fmaxf(hi, fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w)));
     }
     err *= 1.01f;  // what the comparisons below round
     // [lo, hi] holds the m-th largest s~. Unmapped blocks count as the least s~: too much, but never enough to be in for certain.
@@ -366,7 +384,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
     if (err < INFINITY) {
         for (int pass = 0; pass < 3 && hi - lo > 16.f * err; pass++) {
             // s~ above the range (from the second pass on) counts in the top bin: the m-th lies in the range, so its bin is found
-            const float inv = (float)(kSelBins - 1) / (hi - lo);
+            const float range = hi - lo, inv = __fdividef((float)(kSelBins - 1), range), width = range * (1.f / (kSelBins - 1));
             *reinterpret_cast<uint4*>(hist + 4 * tid) = make_uint4(0, 0, 0, 0);
             __syncthreads();
 #pragma unroll 4
@@ -376,8 +394,8 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
             }
             everyone();
             find_bin(hist, ctas, m, red_i, &s_bin, &s_above, &s_in);
-            // the bin's edges, out by more than the index above rounds (2^-22 of the range)
-            const float slack = (hi - lo) * 0x1p-20f, from_s = lo + (float)s_bin / inv - slack, to_s = lo + (float)(s_bin + 1) / inv + slack;
+            // the bin's edges, out by more than the index above and they themselves round (2^-21 of the range)
+            const float slack = range * 0x1p-19f, from_s = fmaf((float)s_bin, width, lo) - slack, to_s = fmaf((float)(s_bin + 1), width, lo) + slack;
             lo = fmaxf(lo, from_s);
             hi = fminf(hi, to_s);
             if (hi - lo > 16.f * err) everyone();  // the histograms have been read: they may be cleared
@@ -585,7 +603,8 @@ extern "C" int b200_paged_select(b200_ctx* ctx, const b200_paged_cache* c, const
     static SmemLimit limit[4];
     int ctas = 1;
     while (ctas < kSelMaxCluster && (long long)r->n_rows * c->n_kv_heads * ctas < 2 * ctx->sm_count && c->max_blocks > kSelRun * ctas) ctas *= 2;
-    const int chunk = ceil_div(c->max_blocks, kSelRun * ctas) * kSelRun;  // of one CTA
+    int chunk = ceil_div(c->max_blocks, kSelRun * ctas) * kSelRun;  // scores a CTA has room for
+    if (chunk < kSelGather) chunk = c->max_blocks < kSelGather ? ceil_div(c->max_blocks, kSelRun) * kSelRun : kSelGather;
     auto smem = [](int blocks) { return (size_t)blocks * 4 + 2 * ((size_t)blocks / 8); };
     CUDA_TRY(ctx, limit[2 * (c->head_dim == 128) + (G <= 4)].raise(kernel, ctx->device, smem(kSelMaxBlocks)));
     launch_cluster(kernel, ctas, dim3((unsigned)(r->n_rows * ctas), c->n_kv_heads), dim3(kSelThreads), smem(chunk), ctx->stream, *c, r->row_slot, r->row_pos, q,
