@@ -437,6 +437,32 @@ def test_attend_queries_of_any_size(ops):
         _close(out, want, worst)
 
 
+def test_attend_softcap_from_the_smallest_to_the_largest_scores(ops):
+    """Sixteen keys of score x against one of score 0: the weights are 16 / (16 + exp(-c)) and the rest, c = cap * tanh(x / cap).
+    tanh is held to 2^-21 of its value, a weight to that of c plus 2^-21 each for exp, the split into two halves and the sums."""
+    hd, br, cap = 64, 16, 8.0
+    x = torch.cat((torch.logspace(-6, 4, 26, dtype=torch.float64), torch.tensor([0.55, 0.5999, 0.6, 0.6001, 0.7]).double() * cap))
+    x = torch.cat((x, -x)).cuda().half()
+    n = len(x)
+    k_pool = torch.zeros(n + 2, 1, br, hd, dtype=torch.float16, device="cuda")
+    v_pool = torch.zeros_like(k_pool)
+    k_pool[1:n + 1, 0, :, 0] = x[:, None]
+    v_pool[1:n + 1, 0, :, 0], v_pool[n + 1, 0, :, 1] = 1.0, 1.0
+    q = torch.zeros(n, hd, device="cuda")
+    q[:, 0] = 1.0
+    table = np.array([[i + 1, n + 1] for i in range(n)], np.int32)
+    cache, packed = _views(ops, table, np.arange(n), np.full(n, br), br, n + 2, k_pool, v_pool)
+    out = torch.empty(n, hd, device="cuda")
+    cache.attend(packed, q, dev(np.tile(np.array([0, 1], np.int32), (n, 1, 1))), out, scale=1.0, softcap=cap)
+    torch.cuda.synchronize()
+    c = cap * torch.tanh(x.double() / cap)
+    want = 16 / (16 + torch.exp(-c))
+    bound = 2.0 ** -21 * c.abs() + 3 * 2.0 ** -21
+    assert ((out[:, 0].double() - want).abs() <= bound * want).all()
+    assert ((out[:, 1].double() - (1 - want)).abs() <= bound * (1 - want)).all()
+    assert out[:, 2:].eq(0).all()
+
+
 def test_attend_offsets_past_32_bits(ops):
     """A pool of more than 2^31 values: the last block lies 4 GB behind the first."""
     kv, G, hd, br = 8, 2, 128, 64
