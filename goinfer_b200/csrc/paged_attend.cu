@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) paged_attend_kernel(const b200
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const int e = (int)(__float_as_uint(most) >> 23) - 127;
-        const int shift = most > 0.f && e < 128 ? max(-100, min(100, e)) : 0;
+        const int shift = most > 0.f && e < 128 ? max(-126, min(126, e)) : 0;
         const float down = gid < G ? __uint_as_float((unsigned)(127 - shift) << 23) : 0.f;
         scale *= __uint_as_float((unsigned)(127 + shift) << 23);
 #pragma unroll

@@ -4,6 +4,7 @@
   python -m goinfer_b200.microbench q4k --rows 1 2 4 8 16 32 256 [--n 12288 --k 4096]
   python -m goinfer_b200.microbench f16 --rows 256 [--n 151936 --k 4096]
   python -m goinfer_b200.microbench prefill --rows 2048 [--pos0 0 --heads 32 --kv-heads 8 --head-dim 128]
+  python -m goinfer_b200.microbench paged --rows 256 [--ctx-lo 128 --ctx-hi 8192 --select 64]   (append, select and attend over torch arrays)
   python -m goinfer_b200.microbench gateup --rows 256 [--f 12288 --k 4096 --mode 1]   (one call through host buffers: for profilers)
 
 Times are CUDA-event averages per launch after warm-up. Weight matrices are cycled through several copies and KV pools
@@ -11,6 +12,50 @@ are far larger than the 126 MB L2, so no launch finds its inputs cached.
 """
 import argparse
 import json
+
+
+def paged(args):
+    """One decode token a sequence over a paged cache in torch's memory: a plan, then a layer's append, select and attend, each
+    timed over `iters` launches with the pools and bounds of a whole batch behind them."""
+    import torch
+    from .ops import Ops
+    from .paged import PagedCache, PagedRows
+    stream = torch.cuda.Stream()
+    ops = Ops(0, stream=stream.cuda_stream)
+    n, br, kv, hd = args.rows, args.block_rows, args.kv_heads, args.head_dim
+    with torch.cuda.stream(stream):
+        i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+        f16 = lambda *s: torch.randn(*s, dtype=torch.float16, device="cuda")  # noqa: E731
+        torch.manual_seed(2)
+        length = torch.linspace(args.ctx_lo, args.ctx_hi, n).round().to(torch.int32)[torch.randperm(n)]
+        blocks = -(-(length + 1) // br)
+        n_blocks = 1 + int(blocks.sum())
+        stack = torch.arange(n_blocks - 1, -1, -1, dtype=torch.int32, device="cuda")
+        k_pool, v_pool = f16(n_blocks, kv, br, hd), f16(n_blocks, kv, br, hd)
+        bounds = torch.stack((k_pool.amin(2), k_pool.amax(2)), 2).contiguous()
+        cache = PagedCache(ops, i32(n, int(blocks.max())), i32(n), stack, i32(1) + (n_blocks - 1), br, k_pool, v_pool, bounds)
+        grow, rows = PagedRows(i32(int(length.sum())), i32(int(length.sum())), i32(int(length.sum())), i32(n + 1), i32(4)), \
+            PagedRows(i32(n), i32(n), i32(n), i32(n + 1), i32(4))
+        length = length.cuda()
+        cache.plan(torch.zeros_like(length), length, grow)
+        one = torch.ones_like(length)
+        k, q = torch.randn(n, kv, hd, device="cuda"), torch.randn(n, args.heads, hd, device="cuda")
+        sel, out = i32(n, kv, args.select), torch.empty_like(q)
+        scored = int((torch.where(blocks > args.select, blocks - 2, 0)).sum()) * kv
+        read = int(torch.minimum(torch.minimum(blocks, torch.tensor(args.select)) * br, length.cpu() + 1).sum()) * kv
+        for name, call, nbytes in (("plan", lambda: cache.plan(length, one, rows), 4 * 9 * n), ("append", lambda: cache.append(rows, k, k), 12 * k.numel()),
+                                   ("select", lambda: cache.select(rows, q, sel), 4 * hd * scored), ("attend", lambda: cache.attend(rows, q, sel, out), 4 * hd * read)):
+            for _ in range(args.warmup):
+                call()
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(args.iters):
+                call()
+            b.record()
+            stream.synchronize()
+            ms = a.elapsed_time(b) / args.iters
+            print(json.dumps({"kernel": "paged " + name, "rows": n, "ms_per_launch": ms, "bytes": nbytes, "GBps": nbytes / ms / 1e6,
+                              "plan_status": rows.status.tolist()}))
 
 
 def main():
@@ -55,7 +100,20 @@ def main():
     u.add_argument("--f", type=int, default=12288)
     u.add_argument("--k", type=int, default=4096)
     u.add_argument("--mode", type=int, default=1, help="0 matmul + SwiGLU kernel, 1 SwiGLU in the matmul's epilogue, 2 interleaved rows + SwiGLU kernel")
+    d = sub.add_parser("paged")
+    d.add_argument("--rows", type=int, default=256)
+    d.add_argument("--ctx-lo", type=int, default=128)
+    d.add_argument("--ctx-hi", type=int, default=8192)
+    d.add_argument("--heads", type=int, default=32)
+    d.add_argument("--kv-heads", type=int, default=8)
+    d.add_argument("--head-dim", type=int, default=128)
+    d.add_argument("--block-rows", type=int, default=16)
+    d.add_argument("--select", type=int, default=64)
+    d.add_argument("--iters", type=int, default=20)
+    d.add_argument("--warmup", type=int, default=3)
     args = ap.parse_args()
+    if args.what == "paged":
+        return paged(args)
     from .ops import Ops
     ops = Ops(0)
     if args.what == "attention":

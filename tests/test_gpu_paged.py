@@ -267,12 +267,16 @@ SELECT_SHAPES = [(1, 2, 1, 64, 16, 300, 1, 1, 8), (5, 3, 2, 128, 16, 70, 1, 1, 9
 
 
 @pytest.mark.parametrize("rows,kv,G,hd,br,max_blocks,n_first,n_recent,n", SELECT_SHAPES)
-@pytest.mark.parametrize("kind", ["spread", "ties"])
+@pytest.mark.parametrize("kind", ["spread", "ties", "outliers"])
 def test_select_takes_the_best_blocks(ops, rows, kv, G, hd, br, max_blocks, n_first, n_recent, n, kind):
     rng = np.random.default_rng(rows * max_blocks + G)
     n_blocks = min(rows * max_blocks + 1, 9000)
     centre, reach = rng.normal(0, 1, (n_blocks, kv, hd)), np.abs(rng.normal(0, 1, (n_blocks, kv, hd)))
     bounds = np.stack((centre - reach, centre + reach), 2).astype(np.float16)
+    if kind == "outliers":  # a few blocks and one dim far off: the range of the scores says little about most of them
+        centre[rng.random(n_blocks) < 0.02] *= 400
+        centre[:, :, 5] *= 30
+        bounds = np.stack((centre - reach, centre + reach), 2).astype(np.float16)
     if kind == "ties":
         bounds = bounds[rng.integers(0, 4, n_blocks)]  # four kinds of blocks: most decisions are ties
     q = rng.normal(0, 1, (rows, kv * G * hd)).astype(np.float32)
@@ -426,7 +430,7 @@ def test_attend_queries_of_any_size(ops):
     torch.manual_seed(4)
     v_pool = torch.randn(5, kv, br, hd, device="cuda").half()
     table, sel = np.array([[1, 2, 3, 4]], np.int32), np.arange(4, dtype=np.int32).reshape(1, 1, 4)
-    for size, key_size, scale in ((1e6, 1.0, 1e-7), (1e20, 1.0, 1e-21), (1e-9, 1.0, 1e8), (3.0, 6e4, 1e-6), (1e-30, 1.0, 1e30), (0.0, 1.0, 1.0)):
+    for size, key_size, scale in ((1e6, 1.0, 1e-7), (1e20, 1.0, 1e-21), (1e-9, 1.0, 1e8), (3.0, 6e4, 1e-6), (1e-30, 1.0, 1e30), (1e-37, 1.0, 1e37), (1e37, 0.1, 1e-36), (0.0, 1.0, 1.0)):
         k_pool = (torch.randn(5, kv, br, hd, device="cuda") * key_size).clamp(-65000, 65000).half()
         q = torch.randn(1, kv * G * hd, device="cuda") * size
         cache, packed = _views(ops, table, [0], [60], br, 5, k_pool, v_pool)
@@ -716,3 +720,14 @@ def test_the_documented_step_runs():
     x = torch.einsum("hgd,khd->hgk", env["q"][r].double().reshape(8, 4, 128), keys.double()) * 128 ** -0.5
     want = torch.einsum("hgk,khd->hgd", torch.softmax(x, -1), values.double()).reshape(32, 128)
     _close(env["out"][r], want, torch.einsum("hgd,khd->hgk", env["q"][r].double().reshape(8, 4, 128).abs(), keys.double().abs()).max().item() * 128 ** -0.5)
+
+
+def test_the_microbenchmark_runs(capsys, monkeypatch):
+    import json
+    import sys
+    from goinfer_b200 import microbench
+    monkeypatch.setattr(sys, "argv", "microbench paged --rows 5 --ctx-lo 40 --ctx-hi 900 --heads 8 --kv-heads 2 --head-dim 64 --select 9 --iters 2".split())
+    microbench.main()
+    lines = [json.loads(line) for line in capsys.readouterr().out.splitlines()]
+    assert [x["kernel"] for x in lines] == ["paged plan", "paged append", "paged select", "paged attend"]
+    assert all(x["plan_status"][:2] == [0, 5] and x["ms_per_launch"] > 0 for x in lines)
