@@ -12,8 +12,8 @@
 //     s~ = sum_{q > 0} q_d hi_d + sum_{q <= 0} q_d lo_d     as mma.sync m16n8k16: 16 blocks x 8 heads x 16 dims,
 // q scaled by a power of two (largest |q| in [1, 2)) and split into fp16 parts hi + 2^-11 lo, products exact, fp32 sums. The
 // split leaves at most 2^-22 |q_d| or 2^-36; a step that adds 16 products to the sum is off by at most 17 * 2^-23 of the terms'
-// absolute sum S, 16 of them by 2^-14.9 S. E = 2^-13 S + 2^-12 covers it (128 dims of the largest fp16 bound times 2^-36 are
-// 2^-13), with S = sum |q_d| max(|lo_d|, |hi_d|), which is no less than the terms' sum, from the same unit. The true m-th
+// absolute sum S, the eight steps of either sum by 2^-15.9 S. E = 2^-14 S + 2^-12 covers it (128 dims of the largest fp16 bound
+// times 2^-36 are 2^-13), with S = sum |q_d| max(|lo_d|, |hi_d|), which is no less than the terms' sum, from the same unit. The true m-th
 // score lies within E of the m-th s~, so a block whose s~ is more than 2E above (below) that is in (out) for certain; only
 // the blocks between (a handful) are scored in f64. An infinity or a NaN anywhere makes E infinite, and every block is
 // scored in f64.
@@ -60,33 +60,15 @@ __device__ __forceinline__ unsigned long long key_of(double s) {
     return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | 0x8000000000000000ull;
 }
 
-// exclusive scan over the block's threads; total in `total`
-__device__ __forceinline__ int block_scan(int v, int* red, int& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int s = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += t;
-    }
-    __syncthreads();
-    if (lane == 31) red[warp] = s;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kSelWarps; w++) {
-        if (w < warp) before += red[w];
-        total += red[w];
-    }
-    return before + s - v;
-}
-
-// Finds the bin in which the running count from the top of the cluster's histogram (the sum of the CTAs') reaches `need`.
-// A thread holds four bins.
-__device__ __forceinline__ void find_bin(const unsigned* hist, int ctas, int need, int* red, int* s_bin, int* s_above, int* s_in) {
-    static_assert(kSelBins == 4 * kSelThreads, "four bins a thread");
-    const int first = kSelBins - 4 - 4 * (int)threadIdx.x;
+// Finds the bin in which the running count from the top of the cluster's histogram (the sum of the CTAs') reaches `need`, and
+// the counts above it and in it. A thread holds four bins.
+struct Found {
+    int bin, above, in;
+};
+__device__ __forceinline__ void find_bin(const unsigned* hist, int ctas, int need, int* red, Found* found) {
+    constexpr int BPT = kSelBins / kSelThreads;
+    static_assert(BPT == 4, "a uint4 a thread");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = kSelBins - BPT * (1 + (int)threadIdx.x);
     uint4 h = make_uint4(0, 0, 0, 0);
     if (ctas == 1) {
         h = *reinterpret_cast<const uint4*>(hist + first);
@@ -97,17 +79,24 @@ __device__ __forceinline__ void find_bin(const unsigned* hist, int ctas, int nee
 #pragma unroll
         for (int w = 0; w < kSelMaxCluster; w++) { h.x += t[w].x; h.y += t[w].y; h.z += t[w].z; h.w += t[w].w; }
     }
-    const int count[4] = {(int)h.w, (int)h.z, (int)h.y, (int)h.x};
+    const int count[BPT] = {(int)h.w, (int)h.z, (int)h.y, (int)h.x};  // from the top
     const int mine = count[0] + count[1] + count[2] + count[3];
-    int total;
-    int above = block_scan(mine, red, total);
+    int above = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, above, o);
+        if (lane >= o) above += t;
+    }
+    if (lane == 31) red[warp] = above;
+    __syncthreads();
+    above -= mine;
+#pragma unroll
+    for (int w = 0; w < kSelWarps; w++) above += w < warp ? red[w] : 0;
     if (above < need && above + mine >= need) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < BPT; j++) {
             if (above < need && above + count[j] >= need) {
-                *s_bin = first + 3 - j;
-                *s_above = above;
-                *s_in = count[j];
+                *found = Found{first + BPT - 1 - j, above, count[j]};
                 above = need;  // found
             } else {
                 above += count[j];
@@ -176,7 +165,8 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
     __shared__ int doubt[kSelDoubt];
     __shared__ int own_doubt[kSelDoubt];
     __shared__ int red_i[kSelWarps];
-    __shared__ int s_bin, s_above, s_in, s_doubt;
+    __shared__ Found found;
+    __shared__ int s_in, s_doubt;  // this CTA's blocks that are in for certain and in doubt
     int ctas = (int)cluster_size();
     const int rank = (int)cluster_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = blockIdx.x / ctas, kvh = blockIdx.y;
@@ -209,6 +199,11 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
         if (lane < ctas) cluster_store(cluster_addr(what, lane), v);
     };
     if (ctas > 1) cluster_arrive();
+    auto clear = [&] {
+        for (int i = 4 * tid; i < kSelBins; i += 4 * kSelThreads) *reinterpret_cast<uint4*>(hist + i) = make_uint4(0, 0, 0, 0);
+    };
+    clear();
+    if (tid == 0) s_in = s_doubt = 0;
     // this CTA's blocks: from .. from + own - 1 of the middle, 16 a warp at a time
     const int chunk = (n + kSelRun * ctas - 1) / (kSelRun * ctas) * kSelRun, from = min(n, rank * chunk);
     int own = min(n, from + chunk) - from;
@@ -279,7 +274,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
         // E is never negative, so its bits order as it does, and an infinity or a NaN (0 * inf) is above every number
         unsigned err_bits = 0;
         float mn = INFINITY, mx = -INFINITY;
-        const float k0 = 0x1p-13f * f0, k1 = 0x1p-13f * f1, floor0 = 0x1p-12f * f0, floor1 = 0x1p-12f * f1;
+        const float k0 = 0x1p-14f * f0, k1 = 0x1p-14f * f1, floor0 = 0x1p-12f * f0, floor1 = 0x1p-12f * f1;
         const uint8_t* bounds = static_cast<const uint8_t*>(c.key_bounds) + (size_t)kvh * 4 * HD + 16 * tig;
         const size_t block_bytes = (size_t)c.n_kv_heads * 4 * HD;
         for (; b0 < own; b0 += kSelRun) {
@@ -385,20 +380,22 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
         for (int pass = 0; pass < 3 && hi - lo > 16.f * err; pass++) {
             // s~ above the range (from the second pass on) counts in the top bin: the m-th lies in the range, so its bin is found
             const float range = hi - lo, inv = __fdividef((float)(kSelBins - 1), range), width = range * (1.f / (kSelBins - 1));
-            *reinterpret_cast<uint4*>(hist + 4 * tid) = make_uint4(0, 0, 0, 0);
-            __syncthreads();
 #pragma unroll 4
             for (int i = tid; i < own; i += kSelThreads) {
                 const float s = score(i);
                 if (s >= lo) atomicAdd(&hist[min(kSelBins - 1, (int)((fminf(s, hi) - lo) * inv))], 1u);
             }
             everyone();
-            find_bin(hist, ctas, m, red_i, &s_bin, &s_above, &s_in);
+            find_bin(hist, ctas, m, red_i, &found);
             // the bin's edges, out by more than the index above and they themselves round (2^-21 of the range)
-            const float slack = range * 0x1p-19f, from_s = fmaf((float)s_bin, width, lo) - slack, to_s = fmaf((float)(s_bin + 1), width, lo) + slack;
+            const float slack = range * 0x1p-19f, from_s = fmaf((float)found.bin, width, lo) - slack, to_s = fmaf((float)(found.bin + 1), width, lo) + slack;
             lo = fmaxf(lo, from_s);
             hi = fminf(hi, to_s);
-            if (hi - lo > 16.f * err) everyone();  // the histograms have been read: they may be cleared
+            if (hi - lo > 16.f * err) {
+                everyone();  // the histograms have been read
+                clear();
+                __syncthreads();
+            }
         }
     } else {
         lo = -INFINITY;
@@ -406,8 +403,6 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
     }
     // in for certain, out for certain, in doubt
     const float sure_in = hi + 2.f * err, sure_out = lo - 2.f * err;
-    if (tid == 0) s_doubt = 0;
-    __syncthreads();
     const int words = (own + 31) >> 5;
     int in = 0;
 #pragma unroll 2
@@ -427,25 +422,27 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
         }
         in += __popc(in_word);
     }
-    if (lane == 0) red_i[warp] = in;
+    if (lane == 0 && in > 0) atomicAdd(&s_in, in);
     __syncthreads();
-    const int n_own = s_doubt;  // this CTA's blocks in doubt
-    if (warp == 0) {
-        in = 0;
-        for (int w = 0; w < kSelWarps; w++) in += red_i[w];
-        tell(n_in + rank, in);
-        tell(n_doubt_of + rank, n_own);
-    }
-    everyone();
-    int need = m, n_doubt = 0, before = 0;  // before: blocks in doubt of the CTAs ahead
-    int first = n_first;                    // this CTA's first place in the list
-    for (int w = 0; w < ctas; w++) {
-        if (w == rank) {
-            before = n_doubt;
-            first += m - need;
+    const int n_own = s_doubt;
+    int need = m - s_in, n_doubt = n_own, before = 0;  // of the cluster; before: blocks in doubt of the CTAs ahead
+    int first = n_first;                               // this CTA's first place in the list
+    if (ctas > 1) {
+        if (warp == 0) {
+            tell(n_in + rank, s_in);
+            tell(n_doubt_of + rank, n_own);
         }
-        need -= n_in[w];
-        n_doubt += n_doubt_of[w];
+        everyone();
+        need = m;
+        n_doubt = 0;
+        for (int w = 0; w < ctas; w++) {
+            if (w == rank) {
+                before = n_doubt;
+                first += m - need;
+            }
+            need -= n_in[w];
+            n_doubt += n_doubt_of[w];
+        }
     }
     // `need`, 1 .. n_doubt, of those in doubt are in
     constexpr int LPB = HD / 8, BPW = 32 / LPB;
@@ -507,15 +504,15 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
             int here;
             while (true) {  // at most four divisions of the range by 512
                 const int width = 32 - __clz((int)(kmax - kmin)), shift = width > 9 ? width - 9 : 0;
-                for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+                clear();
                 __syncthreads();
                 for (int i = tid; i < own; i += kSelThreads)
                     if (in_doubt(i) && key[i] >= kmin && key[i] <= kmax) atomicAdd(&hist[(key[i] - kmin) >> shift], 1u);
                 everyone();
-                find_bin(hist, ctas, need, red_i, &s_bin, &s_above, &s_in);
-                here = s_in;
-                need -= s_above;
-                const unsigned edge = kmin + ((unsigned)s_bin << shift), width_less_1 = (1u << shift) - 1u;
+                find_bin(hist, ctas, need, red_i, &found);
+                here = found.in;
+                need -= found.above;
+                const unsigned edge = kmin + ((unsigned)found.bin << shift), width_less_1 = (1u << shift) - 1u;
                 kmax = kmax - edge < width_less_1 ? kmax : edge + width_less_1;  // (edge + width may pass 2^32)
                 kmin = edge;
                 everyone();  // the histograms have been read
