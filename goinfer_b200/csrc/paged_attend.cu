@@ -59,7 +59,7 @@ struct AttendShape {
 };
 
 // Two CTAs an SM at least: with all the registers that leaves it the compiler keeps more of a tile's steps in flight than it would
-// by itself (4 x 131k keys 45.4 against 49.6 us).
+// by itself (4 x 131k keys 45.6 against 49.7 us; 256 rows 312 against 310).
 template <int HD>
 __global__ void __launch_bounds__(kAttThreads, 2) paged_attend_kernel(const b200_paged_cache c, const int32_t* row_slot,
                                                                    const int32_t* row_pos, const float* q, size_t ldq, int G,
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) paged_attend_kernel(const b200
         __syncwarp();
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    pdl_trigger();  // not before: CTAs of the next kernel beside this one's would lie unevenly (ragged lists 15.0 against 13.3 us)
+    pdl_trigger();  // not before: CTAs of the next kernel beside this one's would lie unevenly (ragged lists 13.9 against 12.9 us)
     __syncthreads();
     // join the warps (in the rings' room): acc[warp][head][dim]; maximum and sum [warp][head] become the warps' factors
     float* acc = reinterpret_cast<float*>(att_smem);

@@ -143,8 +143,8 @@ __device__ __forceinline__ unsigned long long exact_key(const b200_paged_cache& 
     return key_of(ok ? best : -top);
 }
 
-// Four CTAs an SM: the 128 registers this leaves a thread hold a run's bounds (64) on their way; with fewer the compiler starts
-// the products before the last load is out (batch 66 us either way, long contexts 50 against 58 us).
+// Four CTAs an SM: the 128 registers this leaves a thread hold a run's bounds (64) on their way; left to itself the compiler takes
+// fewer and starts the products before the last load is out (batch 66.5 against 57.6 us, long contexts 59.9 against 47.1 us).
 template <int HD, bool NARROW>
 __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200_paged_cache c, const int32_t* row_slot,
                                                                    const int32_t* row_pos, const float* q, size_t ldq, int G,
