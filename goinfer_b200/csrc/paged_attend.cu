@@ -13,8 +13,9 @@
 // fp16 hi + lo parts (x = hi + lo to 2^-22), so the result keeps fp32 accuracy. S[head][key] = Q K^T takes the group's
 // heads as rows; the context is accumulated transposed, O^T[dim][head] = V^T P^T, where a lane's scores are already the
 // second operand. A tile's context starts from zero and is added to the running one by a rounded fma: the matrix unit cuts off
-// what it adds to, and over the tiles of a long list that went one way (2048 keys: 1.5e-6 of the result, 3e-7 so). Rows of the last tile behind the position are filled with zeros by the copy: what the pool holds there
-// (a NaN, say) meets a weight of 0 and must not be multiplied.
+// what it adds to, and over the tiles of a long list that went one way (2048 keys: 1.5e-6 of the result, 4e-7 so). Rows of the
+// last tile behind the position are filled with zeros by the copy: what the pool holds there (a NaN, say) meets a weight of 0
+// and must not be multiplied.
 #include "paged.cuh"
 
 namespace {
@@ -327,8 +328,9 @@ extern "C" int b200_paged_attend(b200_ctx* ctx, const b200_paged_cache* c, const
     if (n_heads < 1 || n_heads % c->n_kv_heads || n_heads / c->n_kv_heads > 8)
         B200_FAIL(ctx, B200_BAD_ARGUMENT, "b200_paged_attend: %d query heads over %d kv heads; a group has 1 to 8 query heads", n_heads, c->n_kv_heads);
     if (n_select < 1 || n_select > kAttMaxList) B200_FAIL(ctx, B200_BAD_ARGUMENT, "b200_paged_attend: lists of %d blocks; 1 to %d", n_select, kAttMaxList);
-    if (!(scale >= 0.f) || !(softcap >= 0.f) || scale > 3.4e38f || softcap > 3.4e38f)
-        B200_FAIL(ctx, B200_BAD_ARGUMENT, "b200_paged_attend: scale %g and softcap %g must be finite and not negative", (double)scale, (double)softcap);
+    if (!(scale >= 0.f) || !(softcap >= 0.f) || scale > 3.4e38f || softcap > 3.4e38f || (softcap > 0.f && softcap < 1e-30f))
+        B200_FAIL(ctx, B200_BAD_ARGUMENT, "b200_paged_attend: scale %g and softcap %g must be finite and not negative, a softcap 0 or at least 1e-30",
+                  (double)scale, (double)softcap);
     if (r->n_rows == 0) return B200_OK;
     const long long width = (long long)n_heads * c->head_dim;
     if (!q || !sel || !out || paged_misaligned(q, 16) || paged_misaligned(sel, 4) || paged_misaligned(out, 16) || ldq < width || (ldq & 3) || ldo < width ||

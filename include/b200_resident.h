@@ -403,7 +403,7 @@ typedef struct {
 int b200_paged_plan(b200_ctx* ctx, const b200_paged_cache* cache, const b200_paged_rows* rows, const int32_t* kv_len, const int32_t* n_new);
 
 /* Stores row r of k and v ([n_rows][ldk or ldv] f32, n_kv_heads * head_dim used, 16-byte aligned, strides a multiple of 4),
- * rounded to fp16, at slot_map[r]; rows whose slot_map is negative or past the pools are left out. With key_bounds, the
+ * rounded to fp16, at slot_map[r]; rows whose slot_map is negative, past the pools or in the null block are left out. With key_bounds, the
  * bounds of every block written to are then those of its rows 0 .. the last one written (rows behind it, left over from a
  * rewound sequence, do not count; a NaN makes its bound NaN). slot_map as plan writes it: distinct, a block's rows next to
  * one another in ascending order. */
@@ -421,7 +421,8 @@ int b200_paged_select(b200_ctx* ctx, const b200_paged_cache* cache, const b200_p
 
 /* Attention of every row over the keys 0 .. row_pos of the blocks that its list names, per kv head: sel as select writes it,
  * or any list of table positions (entries that are negative, or behind the row's position, are left out; one that is named
- * twice counts twice). Scores are scale * q.k (scale 0: 1/sqrt(head_dim)), softcap > 0 caps them (decoder/attention.go:287-295);
+ * twice counts twice). Scores are scale * q.k (scale 0: 1/sqrt(head_dim)), softcap > 0 (at least 1e-30) caps them
+ * (decoder/attention.go:287-295);
  * a row that sees no key gets zeros. q [n_rows][ldq] and out [n_rows][ldo] f32, 16-byte aligned, strides a multiple of 4,
  * out apart from the inputs. fp32 accuracy over the fp16 cache. */
 int b200_paged_attend(b200_ctx* ctx, const b200_paged_cache* cache, const b200_paged_rows* rows, const float* q, int ldq, int n_heads,

@@ -139,7 +139,7 @@ REFUSED = (
                                      dict(first=4), dict(n=0), dict(n=2049), dict(sel=None), dict(sel=A + 2), dict(first=0x7fffffff, recent=0x7fffffff))] +
     [("attend", {}, {}, a) for a in (dict(q=None), dict(q=A + 4), dict(ldq=508), dict(ldq=514), dict(heads=0), dict(heads=7), dict(heads=18, ldq=2048, ldo=2048), dict(n=0), dict(n=2049),
                                      dict(sel=None), dict(sel=A + 2), dict(out=None), dict(out=A + 8), dict(ldo=508), dict(ldo=514), dict(scale=-1.0), dict(scale=NAN),
-                                     dict(scale=INF), dict(cap=-1.0), dict(cap=NAN), dict(cap=INF))])
+                                     dict(scale=INF), dict(cap=-1.0), dict(cap=1e-38), dict(cap=NAN), dict(cap=INF))])
 
 
 @pytest.mark.parametrize("op,cache,rows,args", REFUSED, ids=lambda x: x if isinstance(x, str) else ",".join(f"{k}={v}" for k, v in x.items()) or "-")
