@@ -52,6 +52,32 @@ struct SmemLimit {
 };
 
 #ifdef __CUDACC__
+// How many clusters of 2^lg CTAs of a kernel the GPU holds at once, asked once per device. A cluster stays within one group of
+// SMs, so this is less than the CTAs that fit divided by the cluster's size, by what the groups' sizes leave over: with four
+// CTAs an SM of 148, 71 clusters of 8, not 74. (0 where not even one fits.) One object per kernel, block and `smem`.
+struct ClusterFit {
+    std::atomic<int> known[64][4] = {};  // [device][lg]: the count and one
+    template <typename K>
+    cudaError_t count(K* kernel, int device, int lg, dim3 block, size_t smem, int* n) {
+        if (device < 0 || device >= 64 || lg < 0 || lg > 3) return cudaErrorInvalidValue;
+        const int have = known[device][lg].load(std::memory_order_relaxed);
+        if (have > 0) return *n = have - 1, cudaSuccess;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(1u << lg);
+        cfg.blockDim = block;
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 1u << lg;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(n, kernel, &cfg);
+        if (e == cudaSuccess) known[device][lg].store(*n + 1, std::memory_order_relaxed);
+        return e;
+    }
+};
+
 // launch_pdl (common.cuh: its rule holds here too) with clusters of `cluster` CTAs along x. Every kernel over the paged cache
 // goes through one of the two and waits before it reads anything, so that the launches of a step's calls overlap. What it
 // reads may have been written while it was already resident, so its pointers are not __restrict__: the compiler would turn

@@ -317,6 +317,45 @@ __global__ void __launch_bounds__(kAttThreads, 2) paged_attend_kernel(const b200
     }
 }
 
+// As many CTAs a (row, kv head) as the GPU holds at once (two an SM at head_dim 128, four at 64), each with a tile a warp at
+// least: one more wave costs more than the shorter share saves. Rows x kv heads x tiles, in us with 1, 2, 4, 8 CTAs:
+// 8 x 64: 13.0, 9.4, 6.9, 5.9; 64 x 64: 13.4, 10.0, 8.5, 12.9; 128 x 64: 16.9, 16.5, 20.6, 29.9; 384 x 66: 45, 49, 60, 87.
+// What the GPU holds is asked, not computed: 72 pairs at head_dim 128 (64 blocks of 16) take 13.4 us as clusters of 4 of which
+// 71 fit, 9.6 as clusters of 2.
+//
+// At head_dim 64, with more than two CTAs an SM and no more than three, the launch asks for enough shared memory that a fourth
+// does not fit. The clusters are otherwise placed four to an SM, which leaves a quarter of the SMs idle: 96 pairs x 64 tiles
+// 8.8 -> 7.3 us, 192 pairs with lists of 48 to 66 tiles 12.8 -> 11.9; single CTAs, 440 pairs x 64, 22.1 -> 21.7. Below three an
+// SM it is not worth it (32 pairs, 256 CTAs, 5.7 -> 5.9 with two an SM): the last clusters then no longer fit at once.
+template <int HD>
+int attend_launch(b200_ctx* ctx, const b200_paged_cache& c, const b200_paged_rows& r, const float* q, size_t ldq, int n_heads, float scale, float cap,
+                  const int32_t* sel, int n_select, float* out, size_t ldo) {
+    using S = AttendShape<HD>;
+    constexpr size_t most = S::smem(kAttMaxList), three = 56 * 1024;  // of 228 KB an SM
+    static_assert(HD == 128 || most < three, "");
+    static SmemLimit limit;
+    static ClusterFit fits, fits_three;
+    auto kernel = paged_attend_kernel<HD>;
+    CUDA_TRY(ctx, limit.raise(kernel, ctx->device, most > three ? most : three));
+    const long long pairs = (long long)r.n_rows * c.n_kv_heads;
+    const int tiles = n_select * (c.block_rows / 16);
+    int lg = 0;
+    for (int fit = 0; (kAttMaxCluster >> lg) > 1 && tiles >= (2 * kAttWarps) << lg; lg++) {
+        CUDA_TRY(ctx, fits.count(kernel, ctx->device, lg + 1, dim3(kAttThreads), most, &fit));
+        if (pairs > fit) break;
+    }
+    size_t smem = S::smem(n_select);
+    if (HD == 64 && pairs << lg > 2ll * ctx->sm_count) {
+        int fit = 0;
+        CUDA_TRY(ctx, fits_three.count(kernel, ctx->device, lg, dim3(kAttThreads), three, &fit));
+        if (pairs <= fit) smem = three;
+    }
+    launch_cluster(kernel, 1 << lg, dim3((unsigned)(r.n_rows << lg), c.n_kv_heads), dim3(kAttThreads), smem, ctx->stream, c, r.row_slot, r.row_pos, q, ldq,
+                   n_heads / c.n_kv_heads, scale, cap, sel, n_select, out, ldo);
+    LAUNCH_CHECK(ctx);
+    return B200_OK;
+}
+
 }  // namespace
 
 extern "C" int b200_paged_attend(b200_ctx* ctx, const b200_paged_cache* c, const b200_paged_rows* r, const float* q, int ldq, int n_heads, float scale,
@@ -341,25 +380,7 @@ extern "C" int b200_paged_attend(b200_ctx* ctx, const b200_paged_cache* c, const
     if (ctx->device < 0) B200_FAIL(ctx, B200_CUDA_ERROR, "b200_paged_attend: the context has no device");
     DeviceScope dev;
     CUDA_TRY(ctx, dev.enter(ctx->device));
-    const int G = n_heads / c->n_kv_heads, tiles = n_select * (c->block_rows / 16);
     const float s = scale != 0.f ? scale : 1.0f / sqrtf((float)c->head_dim);
-    // As many CTAs a (row, kv head) as fit the GPU at once (two an SM at head_dim 128, four at 64), each with a tile a warp at
-    // least: one more wave costs more than the shorter share saves. Rows x kv heads x tiles, in us with 1, 2, 4, 8 CTAs:
-    // 8 x 64: 13.0, 9.4, 6.9, 5.9; 64 x 64: 13.4, 10.0, 8.5, 12.9; 128 x 64: 16.9, 16.5, 20.6, 29.9; 384 x 66: 45, 49, 60, 87.
-    int ctas = 1;
-    const int at_once = (c->head_dim == 128 ? 2 : 4) * ctx->sm_count;
-    while (ctas < kAttMaxCluster && 2ll * r->n_rows * c->n_kv_heads * ctas <= at_once && tiles >= 2 * kAttWarps * ctas) ctas *= 2;
-    const dim3 grid((unsigned)(r->n_rows * ctas), c->n_kv_heads);
-    static SmemLimit limit[2];
-    if (c->head_dim == 128) {
-        CUDA_TRY(ctx, limit[1].raise(paged_attend_kernel<128>, ctx->device, AttendShape<128>::smem(kAttMaxList)));
-        launch_cluster(paged_attend_kernel<128>, ctas, grid, dim3(kAttThreads), AttendShape<128>::smem(n_select), ctx->stream, *c, r->row_slot,
-                       r->row_pos, q, (size_t)ldq, G, s, softcap, sel, n_select, out, (size_t)ldo);
-    } else {
-        CUDA_TRY(ctx, limit[0].raise(paged_attend_kernel<64>, ctx->device, AttendShape<64>::smem(kAttMaxList)));
-        launch_cluster(paged_attend_kernel<64>, ctas, grid, dim3(kAttThreads), AttendShape<64>::smem(n_select), ctx->stream, *c, r->row_slot,
-                       r->row_pos, q, (size_t)ldq, G, s, softcap, sel, n_select, out, (size_t)ldo);
-    }
-    LAUNCH_CHECK(ctx);
-    return B200_OK;
+    if (c->head_dim == 128) return attend_launch<128>(ctx, *c, *r, q, (size_t)ldq, n_heads, s, softcap, sel, n_select, out, (size_t)ldo);
+    return attend_launch<64>(ctx, *c, *r, q, (size_t)ldq, n_heads, s, softcap, sel, n_select, out, (size_t)ldo);
 }

@@ -9,6 +9,9 @@ running rescale and by the fp32 sums (u each); numerator and denominator both ca
 2 * u * (2 X + 1 + X + 3) = u * (6 X + 8); the largest single deviation is held to eight times that of the row's rms."""
 import ctypes as C
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -366,7 +369,10 @@ def _close(got, want, worst):
 
 ATTEND_SHAPES = [(1, 1, 1, 64, 16, 1, 1, 0.0), (1, 8, 4, 128, 16, 500, 64, 0.0), (3, 2, 2, 128, 48, 30, 7, 0.0), (5, 1, 3, 64, 256, 4, 4, 20.0),
                  (4, 2, 5, 128, 16, 40, 33, 0.0), (2, 3, 6, 64, 32, 25, 25, 5.0), (9, 1, 7, 128, 64, 9, 6, 0.0), (33, 8, 8, 128, 16, 20, 12, 0.0),
-                 (200, 4, 8, 64, 32, 12, 5, 0.0), (1, 1, 2, 128, 16, 2048, 2048, 0.0)]
+                 (200, 4, 8, 64, 32, 12, 5, 0.0), (1, 1, 2, 128, 16, 2048, 2048, 0.0),
+                 # clusters of 8 (three and four an SM), 4, 2, and single CTAs at head_dim 64; of 4 and 2 at 128
+                 (12, 4, 4, 64, 16, 80, 64, 0.0), (17, 4, 2, 64, 16, 80, 64, 0.0), (20, 4, 3, 64, 16, 80, 64, 7.0), (40, 4, 4, 64, 32, 40, 33, 0.0),
+                 (90, 4, 2, 64, 16, 40, 30, 0.0), (8, 8, 4, 128, 16, 80, 64, 0.0), (9, 8, 2, 128, 16, 80, 64, 0.0)]
 
 
 @pytest.mark.parametrize("rows,kv,G,hd,br,max_blocks,n,cap", ATTEND_SHAPES)
@@ -640,6 +646,41 @@ def test_the_four_operators_as_a_decode_step(ops, replay):
     _run(step, 11, replay)
 
 
+def test_the_first_call_of_a_process_may_be_captured(tmp_path):
+    """Whatever a kernel asks of the device once (limits, how many clusters fit) is allowed while a stream captures."""
+    prog = tmp_path / "first.py"
+    prog.write_text("""
+import torch
+from goinfer_b200.ops import Ops
+from goinfer_b200.paged import PagedCache, PagedRows
+rows, kv, G, hd, br, n = 20, 4, 2, 64, 16, 32
+side = torch.cuda.Stream()
+ops = Ops(0, stream=side.cuda_stream)
+i32 = dict(dtype=torch.int32, device="cuda")
+k, v = (torch.randn(rows * n + 1, kv, br, hd, device="cuda").half() for _ in range(2))
+bounds = torch.zeros(rows * n + 1, kv, 2, hd, dtype=torch.float16, device="cuda")
+table = torch.arange(1, rows * n + 1, **i32).reshape(rows, n)
+packed = PagedRows(torch.arange(rows, **i32), torch.full((rows,), n * br - 1, **i32), torch.zeros(rows, **i32))
+cache = PagedCache(ops, table, torch.full((rows,), n, **i32), torch.zeros(rows * n + 1, **i32), torch.zeros(1, **i32), br, k, v, bounds)
+q, sel = torch.randn(rows, kv * G * hd, device="cuda"), torch.empty(rows, kv, n, **i32)
+outs = [torch.zeros(rows, kv * G * hd, device="cuda") for _ in range(2)]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    cache.select(packed, q, sel, n_first=1, n_recent=1)
+    cache.attend(packed, q, sel, outs[0])
+graph.replay()
+torch.cuda.synchronize()
+with torch.cuda.stream(side):
+    cache.attend(packed, q, sel, outs[1])
+torch.cuda.synchronize()
+assert outs[0].abs().sum() > 0 and torch.equal(outs[0], outs[1])
+""")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, str(prog)], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
+
+
 def test_two_captured_steps_at_once_share_nothing(ops):
     """Two steps' graphs replayed on two streams without an order between them give what each gives alone, bit for bit."""
     alone = []
@@ -699,7 +740,6 @@ def test_a_full_list_gives_dense_attention(ops):
 
 def test_the_documented_step_runs():
     """The step of the integration guide, as it stands there, over two steps of eight sequences."""
-    import os
     text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")).read()
     code = text[text.index("import torch\nfrom goinfer_b200.ops import Ops\nfrom goinfer_b200.paged"):]
     setup, step = code[:code.index("```")].split("layers[0].plan", 1)
