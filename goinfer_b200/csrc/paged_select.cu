@@ -36,6 +36,11 @@ constexpr int kSelDoubt = 256;        // blocks in doubt that are ranked in a li
 constexpr int kSelMaxCluster = 8;
 constexpr int kSelGather = 512;       // room for as many scores costs a CTA little, and the choice among them is quick
 constexpr int kSelRun = 16 * kSelWarps;  // blocks a CTA scores at a time
+// Dynamic shared memory with which four CTAs fit the 228 KB of an SM, and with which three do but not four (head_dim 64, 128). A CTA
+// has 12 to 14 KB of static shared memory, or 17 to 21, and 1 KB that the system keeps. Three stay within 196 KB, so that the L1
+// cache keeps 60: at 208 KB it has 28, and what a row's loads share no longer stays in it (head_dim 128, a group of 8, 320 pairs
+// of 500 blocks 38 against 26 us).
+constexpr size_t kSelFour = 35 * 1024, kSelThree[2] = {46 * 1024, 40 * 1024};
 
 __device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -597,14 +602,37 @@ extern "C" int b200_paged_select(b200_ctx* ctx, const b200_paged_cache* c, const
     const int G = n_heads / c->n_kv_heads;
     auto kernel = c->head_dim == 128 ? (G <= 4 ? paged_select_kernel<128, true> : paged_select_kernel<128, false>)
                                      : (G <= 4 ? paged_select_kernel<64, true> : paged_select_kernel<64, false>);
+    const int variant = 2 * (c->head_dim == 128) + (G <= 4);
+    const long long pairs = (long long)r->n_rows * c->n_kv_heads;
+    auto chunk_of = [&](int ctas) {  // scores a CTA has room for
+        const int chunk = ceil_div(c->max_blocks, kSelRun * ctas) * kSelRun;
+        return chunk >= kSelGather ? chunk : c->max_blocks < kSelGather ? ceil_div(c->max_blocks, kSelRun) * kSelRun : kSelGather;
+    };
+    auto smem_of = [](int blocks) { return (size_t)blocks * 4 + 2 * ((size_t)blocks / 8); };
     static SmemLimit limit[4];
-    int ctas = 1;
-    while (ctas < kSelMaxCluster && (long long)r->n_rows * c->n_kv_heads * ctas < 2 * ctx->sm_count && c->max_blocks > kSelRun * ctas) ctas *= 2;
-    int chunk = ceil_div(c->max_blocks, kSelRun * ctas) * kSelRun;  // scores a CTA has room for
-    if (chunk < kSelGather) chunk = c->max_blocks < kSelGather ? ceil_div(c->max_blocks, kSelRun) * kSelRun : kSelGather;
-    auto smem = [](int blocks) { return (size_t)blocks * 4 + 2 * ((size_t)blocks / 8); };
-    CUDA_TRY(ctx, limit[2 * (c->head_dim == 128) + (G <= 4)].raise(kernel, ctx->device, smem(kSelMaxBlocks)));
-    launch_cluster(kernel, ctas, dim3((unsigned)(r->n_rows * ctas), c->n_kv_heads), dim3(kSelThreads), smem(chunk), ctx->stream, *c, r->row_slot, r->row_pos, q,
+    static ClusterFit fits[4][2], fits_three[4];
+    CUDA_TRY(ctx, limit[variant].raise(kernel, ctx->device, smem_of(kSelMaxBlocks)));
+    // CTAs a (row, kv head): doubled until there are two an SM, as long as the GPU holds all clusters at once and each CTA has
+    // blocks to score. 72 pairs of 500 blocks take 13.3 us as clusters of 8, of which 71 fit, 10.9 as clusters of 4; 144 pairs
+    // of 1875 blocks at head_dim 64 33.5 as clusters of 4, 27.2 as pairs.
+    int lg = 0;
+    for (int fit = 0; (kSelMaxCluster >> lg) > 1 && pairs << lg < 2ll * ctx->sm_count && c->max_blocks > kSelRun << lg; lg++) {
+        const bool roomy = smem_of(chunk_of(2 << lg)) > kSelFour;
+        CUDA_TRY(ctx, fits[variant][roomy].count(kernel, ctx->device, lg + 1, dim3(kSelThreads), roomy ? smem_of(kSelMaxBlocks / 2) : kSelFour, &fit));
+        if (pairs > fit) break;
+    }
+    // Clusters are placed four to an SM, which with three CTAs for each leaves a quarter of the SMs idle. Where the GPU holds them
+    // so, the launch asks for shared memory that keeps a fourth out: 160 pairs of 250 blocks 10.8 -> 9.8 us, of 500 15.1 -> 13.5;
+    // 40 pairs of 1875 17.4 -> 15.5; single CTAs, 440 pairs of 1875, 89 -> 79 us.
+    const int chunk = chunk_of(1 << lg);
+    const size_t three = kSelThree[c->head_dim == 128];
+    size_t smem = smem_of(chunk);
+    if (pairs << lg > 2ll * ctx->sm_count && smem < three) {
+        int fit = 0;
+        CUDA_TRY(ctx, fits_three[variant].count(kernel, ctx->device, lg, dim3(kSelThreads), three, &fit));
+        if (pairs <= fit) smem = three;
+    }
+    launch_cluster(kernel, 1 << lg, dim3((unsigned)(r->n_rows << lg), c->n_kv_heads), dim3(kSelThreads), smem, ctx->stream, *c, r->row_slot, r->row_pos, q,
                    (size_t)ldq, G, n_first, n_recent, n_select, chunk, sel);
     LAUNCH_CHECK(ctx);
     return B200_OK;

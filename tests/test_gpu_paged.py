@@ -266,7 +266,10 @@ def _views(ops, table, slot, pos, br, n_blocks, k_pool=None, v_pool=None, key_bo
 
 SELECT_SHAPES = [(1, 2, 1, 64, 16, 300, 1, 1, 8), (5, 3, 2, 128, 16, 70, 1, 1, 9), (2, 1, 3, 64, 48, 700, 0, 1, 33), (3, 2, 4, 128, 32, 2100, 2, 3, 256),
                  (40, 8, 4, 128, 16, 90, 1, 1, 64), (4, 1, 5, 64, 16, 129, 1, 2, 3), (3, 1, 6, 128, 64, 65, 3, 4, 64), (2, 2, 7, 128, 16, 333, 1, 1, 2),
-                 (7, 2, 8, 128, 16, 530, 1, 1, 100), (1, 1, 8, 64, 16, 5000, 1, 1, 2048), (300, 1, 1, 64, 16, 12, 1, 1, 5), (1, 1, 2, 64, 16, 24576, 1, 1, 700)]
+                 (7, 2, 8, 128, 16, 530, 1, 1, 100), (1, 1, 8, 64, 16, 5000, 1, 1, 2048), (300, 1, 1, 64, 16, 12, 1, 1, 5), (1, 1, 2, 64, 16, 24576, 1, 1, 700),
+                 # clusters of 8 with three CTAs an SM, of 4 where those of 8 do not fit, pairs, and single CTAs
+                 (12, 4, 8, 64, 16, 600, 1, 2, 40), (18, 4, 2, 64, 16, 600, 2, 1, 40), (9, 8, 4, 128, 16, 520, 1, 1, 30), (20, 8, 5, 128, 16, 130, 1, 1, 24),
+                 (40, 8, 2, 128, 16, 70, 0, 1, 9), (300, 1, 8, 64, 32, 66, 1, 1, 9)]
 
 
 @pytest.mark.parametrize("rows,kv,G,hd,br,max_blocks,n_first,n_recent,n", SELECT_SHAPES)
