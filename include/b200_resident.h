@@ -424,7 +424,8 @@ int b200_paged_select(b200_ctx* ctx, const b200_paged_cache* cache, const b200_p
  * twice counts twice). Scores are scale * q.k (scale 0: 1/sqrt(head_dim)), softcap > 0 (at least 1e-30) caps them
  * (decoder/attention.go:287-295);
  * a row that sees no key gets zeros. q [n_rows][ldq] and out [n_rows][ldo] f32, 16-byte aligned, strides a multiple of 4,
- * out apart from the inputs. fp32 accuracy over the fp16 cache. */
+ * out apart from the inputs. fp32 accuracy over the fp16 cache. The same call on the same GPU gives the same bits; a list is
+ * split by the number of rows and by what the GPU holds at once, so in a batch of another size a row's last bits may differ. */
 int b200_paged_attend(b200_ctx* ctx, const b200_paged_cache* cache, const b200_paged_rows* rows, const float* q, int ldq, int n_heads,
                       float scale, float softcap, const int32_t* sel, int n_select, float* out, int ldo);
 
