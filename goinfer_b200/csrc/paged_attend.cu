@@ -10,18 +10,26 @@
 // several streams share nothing.
 //
 // Products run on mma.sync m16n8k16 over the fp16 cache with fp32 accumulation; f32 queries and weights are split into
-// fp16 hi + lo parts (x = hi + lo to 2^-22), so the result keeps fp32 accuracy. S[head][key] = Q K^T takes the group's
-// heads as rows; the context is accumulated transposed, O^T[dim][head] = V^T P^T, where a lane's scores are already the
+// fp16 hi + lo parts. S[head][key] = Q K^T takes the group's heads as rows; the context is accumulated transposed, O^T[dim][head] = V^T P^T, where a lane's scores are already the
 // second operand. A tile's context starts from zero and is added to the running one by a rounded fma: the matrix unit cuts off
 // what it adds to, and over the tiles of a long list that went one way (2048 keys: 1.5e-6 of the result, 4e-7 so). Rows of the
 // last tile behind the position are filled with zeros by the copy: what the pool holds there (a NaN, say) meets a weight of 0
 // and must not be multiplied.
+//
+// Weights. hi + lo is x to 2^-22 where the step of fp16's subnormals, 2^-24, is no more than 2^-21 of x: for x >= 2^-3. A weight is
+// taken in 2^-15ths, p = 2^15 exp(x - m) <= 32768, in the context and in the sum alike, so this holds for those down to 2^-18 of the
+// largest one that the warp has seen. Where a tile has smaller ones (a key 12.5 above the rest, say, whose own value may be
+// next to nothing), they are left out of the first product and multiplied by V again, 2^18 times as large, until none is left: every
+// weight keeps its 2^-22 down to the smallest numbers of fp32. The look costs 1 % at head_dim 128 and nothing at 64 (256 rows of 128
+// blocks 312.6 -> 313.5 us, 45 ragged rows 11.9 either way); where every tile has such weights, the second product takes 329 us in place of
+// 313, 14 in place of 12.
 #include "paged.cuh"
 
 namespace {
 
 constexpr int kAttWarps = 4, kAttThreads = 32 * kAttWarps, kAttStages = 2;
 constexpr int kAttMaxList = 2048;
+constexpr float kWeight = 0x1p15f, kSmall = 0x1p-3f, kStep = 0x1p18f;  // of the weights, see above
 constexpr int kAttMaxCluster = 8;
 
 __device__ __forceinline__ void ldm4(unsigned addr, unsigned (&r)[4]) {
@@ -60,9 +68,10 @@ struct AttendShape {
 };
 
 // Two CTAs an SM at least: with all the registers that leaves it the compiler keeps more of a tile's steps in flight than it would
-// by itself (4 x 131k keys 45.6 against 49.7 us; 256 rows 312 against 310).
+// by itself (4 x 131k keys 45.6 against 49.7 us; 256 rows 312 against 310). Four at head_dim 64: 128 registers, where the compiler takes
+// 137 by itself (128 rows of 64 blocks 25.1 against 27.7 us).
 template <int HD>
-__global__ void __launch_bounds__(kAttThreads, 2) paged_attend_kernel(const b200_paged_cache c, const int32_t* row_slot,
+__global__ void __launch_bounds__(kAttThreads, HD == 64 ? 4 : 2) paged_attend_kernel(const b200_paged_cache c, const int32_t* row_slot,
                                                                    const int32_t* row_pos, const float* q, size_t ldq, int G,
                                                                    float scale, float cap, const int32_t* sel, int n_select,
                                                                    float* out, size_t ldo) {
@@ -218,18 +227,21 @@ __global__ void __launch_bounds__(kAttThreads, 2) paged_attend_kernel(const b200
         const float m_ref = m_new == -INFINITY ? 0.f : m_new;  // nothing seen yet: every weight is exp(-inf) = 0
         const float alpha = __expf(m_run - m_ref);
         float p[4], ps = 0.f;
+        bool small = false;  // a weight that two halves do not hold to 2^-22
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            p[i] = __expf(x[i] - m_ref);
+            p[i] = kWeight * __expf(x[i] - m_ref);
             ps += p[i];
+            small |= p[i] > 0.f && p[i] < kSmall;
         }
+        small = __any_sync(0xffffffffu, small);
         ps += __shfl_xor_sync(0xffffffffu, ps, 1);
         ps += __shfl_xor_sync(0xffffffffu, ps, 2);
         l_run = l_run * alpha + ps;
         m_run = m_new;
         unsigned ph0, pl0, ph1, pl1;
-        split2(p[0], p[1], ph0, pl0);
-        split2(p[2], p[3], ph1, pl1);
+        split2(p[0] < kSmall ? 0.f : p[0], p[1] < kSmall ? 0.f : p[1], ph0, pl0);
+        split2(p[2] < kSmall ? 0.f : p[2], p[3] < kSmall ? 0.f : p[3], ph1, pl1);
         const float a0 = __shfl_sync(0xffffffffu, alpha, (2 * tig) * 4), a1 = __shfl_sync(0xffffffffu, alpha, (2 * tig + 1) * 4);
 #pragma unroll
         for (int mt = 0; mt < KS; mt++) {
@@ -242,6 +254,32 @@ __global__ void __launch_bounds__(kAttThreads, 2) paged_attend_kernel(const b200
             o[mt][1] = fmaf(o[mt][1], a1, d[1]);
             o[mt][2] = fmaf(o[mt][2], a0, d[2]);
             o[mt][3] = fmaf(o[mt][3], a1, d[3]);
+        }
+        for (float down = 1.f; small;) {  // at most eight times: 2^-149 * 2^15 is then above 2^-3
+            down *= 1.f / kStep;
+            bool here = false;
+            small = false;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                p[i] = p[i] < kSmall ? p[i] * kStep : 0.f;  // (those of the step before are done, a NaN was in the first)
+                here |= p[i] >= kSmall;
+                small |= p[i] > 0.f && p[i] < kSmall;
+            }
+            here = __any_sync(0xffffffffu, here);
+            small = __any_sync(0xffffffffu, small);
+            if (!here) continue;
+            split2(p[0] < kSmall ? 0.f : p[0], p[1] < kSmall ? 0.f : p[1], ph0, pl0);
+            split2(p[2] < kSmall ? 0.f : p[2], p[3] < kSmall ? 0.f : p[3], ph1, pl1);
+#pragma unroll
+            for (int mt = 0; mt < KS; mt++) {
+                unsigned v[4];
+                ldm4_t(vb + (unsigned)(lrow * ROWB + (((2 * mt + lsel) ^ (lrow & 7)) << 4)), v);
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816(d, v[0], v[1], v[2], v[3], pl0, pl1);
+                mma16816(d, v[0], v[1], v[2], v[3], ph0, ph1);
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[mt][i] = fmaf(d[i], down, o[mt][i]);
+            }
         }
         __syncwarp();
     }
