@@ -10,7 +10,9 @@
 // several streams share nothing.
 //
 // Products run on mma.sync m16n8k16 over the fp16 cache with fp32 accumulation; f32 queries and weights are split into
-// fp16 hi + lo parts. S[head][key] = Q K^T takes the group's heads as rows; the context is accumulated transposed, O^T[dim][head] = V^T P^T, where a lane's scores are already the
+// fp16 hi + lo parts. S[head][key] = Q K^T takes the group's heads as rows, the lo parts 2^11 times as large and in a sum of their
+// own: with the head's largest |q| in [1, 2), a query keeps its 2^-22 down to 2^-14 and 2^-36 below, so that a small one still
+// counts against a key of thousands; the context is accumulated transposed, O^T[dim][head] = V^T P^T, where a lane's scores are already the
 // second operand. A tile's context starts from zero and is added to the running one by a rounded fma: the matrix unit cuts off
 // what it adds to, and over the tiles of a long list that went one way (2048 keys: 1.5e-6 of the result, 4e-7 so). Rows of the
 // last tile behind the position are filled with zeros by the copy: what the pool holds there (a NaN, say) meets a weight of 0
@@ -47,10 +49,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1
 __device__ __forceinline__ void copy16(unsigned dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo) {
+// x and y as fp16 hi + lo / up
+__device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo, float up = 1.f) {
     const __half2 h = __floats2half2_rn(x, y);
     const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    const __half2 l = __floats2half2_rn((x - f.x) * up, (y - f.y) * up);
     hi = *reinterpret_cast<const unsigned*>(&h);
     lo = *reinterpret_cast<const unsigned*>(&l);
 }
@@ -167,8 +170,8 @@ __global__ void __launch_bounds__(kAttThreads, HD == 64 ? 4 : 2) paged_attend_ke
 #pragma unroll
     for (int s = 0; s < kAttStages - 1; s++) issue(s);
 
-    // the head's largest |q| is brought to [1, 2) by a power of two, which the scale gives back: neither a query beyond fp16's
-    // range nor one among its subnormals loses anything
+    // the head's largest |q| is brought to [1, 2) by a power of two, which the scale gives back: queries may lie beyond fp16's range
+    // or among its subnormals
     unsigned qh0[KS], qh2[KS], ql0[KS], ql2[KS];
     {
         float most = 0.f;
@@ -183,8 +186,8 @@ __global__ void __launch_bounds__(kAttThreads, HD == 64 ? 4 : 2) paged_attend_ke
         scale *= __uint_as_float((unsigned)(127 + shift) << 23);
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
-            split2(qa[ks].x * down, qa[ks].y * down, qh0[ks], ql0[ks]);
-            split2(qb[ks].x * down, qb[ks].y * down, qh2[ks], ql2[ks]);
+            split2(qa[ks].x * down, qa[ks].y * down, qh0[ks], ql0[ks], 0x1p11f);
+            split2(qb[ks].x * down, qb[ks].y * down, qh2[ks], ql2[ks], 0x1p11f);
         }
     }
     float o[KS][4];
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(kAttThreads, HD == 64 ? 4 : 2) paged_attend_ke
             mma16816(s0l, ql0[ks], 0u, ql2[ks], 0u, b[0], b[1]);
             mma16816(s1l, ql0[ks], 0u, ql2[ks], 0u, b[2], b[3]);
         }
-        float x[4] = {s0h[0] + s0l[0], s0h[1] + s0l[1], s1h[0] + s1l[0], s1h[1] + s1l[1]};
+        float x[4] = {fmaf(s0l[0], 0x1p-11f, s0h[0]), fmaf(s0l[1], 0x1p-11f, s0h[1]), fmaf(s1l[0], 0x1p-11f, s1h[0]), fmaf(s1l[1], 0x1p-11f, s1h[1])};
         const int kk[4] = {key0 + 2 * tig, key0 + 2 * tig + 1, key0 + 8 + 2 * tig, key0 + 9 + 2 * tig};
         float mx = -INFINITY;
 #pragma unroll

@@ -82,3 +82,28 @@ def test_attend_weights_of_every_size(ops, rows, kv, G, hd, br, n):  # noqa: F81
     bound = U * (11 * X + 20)
     assert ((out.double() - want).abs() <= bound * want + keys * 2.0 ** -125).all(), (((out.double() - want).abs() / want.clamp_min(1e-35)).max().item(), bound)
     assert (out[want > keys * 2.0 ** -124] > 0).all()
+
+
+@pytest.mark.parametrize("rows,kv,G,hd,br,n", SINK_SHAPES)
+@pytest.mark.parametrize("small", [1e-3, 1e-5, 1e-7])
+def test_attend_small_queries_against_large_keys(ops, rows, kv, G, hd, br, n, small):  # noqa: F811
+    """One dim of the keys is thousands of times the others, and the query is `small` there. A query is kept to 2^-36 of the head's
+    largest where that is more than 2^-22 of it: a score may be off by F = 2^-36 max|q| scale sum |k| besides, the maximum too, and both enter
+    numerator and denominator."""
+    torch.manual_seed(rows + 7 * n)
+    keys = n * br
+    k = (torch.randn(rows * n + 1, kv, br, hd, device="cuda") * 0.05).half()
+    k[..., 9] = ((torch.rand(rows * n + 1, kv, br, device="cuda") * 2 - 1) * 6e4).half()
+    v = (1 + torch.rand(rows * n + 1, kv, br, hd, device="cuda")).half()
+    table = np.arange(1, rows * n + 1, dtype=np.int32).reshape(rows, n)
+    q = torch.randn(rows, kv, G, hd, device="cuda")
+    q[..., 9] = small * (1 + torch.rand(rows, kv, G, device="cuda"))
+    cache, packed = _views(ops, table, np.arange(rows), np.full(rows, keys - 1), br, rows * n + 1, k, v)
+    out = torch.empty(rows, kv, G, hd, device="cuda")
+    cache.attend(packed, q, dev(np.tile(np.arange(n, dtype=np.int32), (rows, kv, 1))), out, scale=0.125)
+    torch.cuda.synchronize()
+    flat = lambda a: a[dev(table).long()].transpose(1, 2).reshape(rows, kv, keys, hd)  # noqa: E731
+    want, X = _exact(q, flat(k), flat(v), 0.125)
+    F = 2.0 ** -36 * q.abs().max().item() * 0.125 * k.double().abs().sum(-1).max().item()
+    err, bound = ((out.double() - want).abs() / want).max().item(), U * (11 * X + 20) + 4 * F
+    assert err <= bound, (err, bound)
