@@ -214,7 +214,9 @@ __global__ void __launch_bounds__(kAttThreads, HD == 64 ? 4 : 2) paged_attend_ke
             mma16816(s0l, ql0[ks], 0u, ql2[ks], 0u, b[0], b[1]);
             mma16816(s1l, ql0[ks], 0u, ql2[ks], 0u, b[2], b[3]);
         }
-        float x[4] = {fmaf(s0l[0], 0x1p-11f, s0h[0]), fmaf(s0l[1], 0x1p-11f, s0h[1]), fmaf(s1l[0], 0x1p-11f, s1h[0]), fmaf(s1l[1], 0x1p-11f, s1h[1])};
+        // (a score that is infinite says so in its upper part; the lower one, of any sign or zero times infinity, says nothing)
+        auto joined = [](float hi, float lo) { return fabsf(hi) == INFINITY ? hi : fmaf(lo, 0x1p-11f, hi); };
+        float x[4] = {joined(s0h[0], s0l[0]), joined(s0h[1], s0l[1]), joined(s1h[0], s1l[0]), joined(s1h[1], s1l[1])};
         const int kk[4] = {key0 + 2 * tig, key0 + 2 * tig + 1, key0 + 8 + 2 * tig, key0 + 9 + 2 * tig};
         float mx = -INFINITY;
 #pragma unroll

@@ -107,3 +107,38 @@ def test_attend_small_queries_against_large_keys(ops, rows, kv, G, hd, br, n, sm
     F = 2.0 ** -36 * q.abs().max().item() * 0.125 * k.double().abs().sum(-1).max().item()
     err, bound = ((out.double() - want).abs() / want).max().item(), U * (11 * X + 20) + 4 * F
     assert err <= bound, (err, bound)
+
+
+@pytest.mark.parametrize("rows,kv,G,hd,br,n", SINK_SHAPES)
+def test_attend_keys_of_minus_infinity(ops, rows, kv, G, hd, br, n):  # noqa: F811
+    """A key value below -65520 is stored as -inf; against a query above zero its score is -inf and its weight 0. A row whose keys
+    all are so has no weight and gives 0; one key at +inf gives NaN, as inf - inf does."""
+    torch.manual_seed(rows + 3 * n)
+    keys = n * br
+    k = torch.randn(rows * n + 1, kv, br, hd, device="cuda").half()
+    v = (1 + torch.rand(rows * n + 1, kv, br, hd, device="cuda")).half()
+    table = np.arange(1, rows * n + 1, dtype=np.int32).reshape(rows, n)
+    k[..., 7] = torch.where(torch.rand(k.shape[:-1], device="cuda") < 0.4, -np.inf, k[..., 7].float()).half()
+    k[..., 2::4, 11] = -np.inf
+    k[..., ::4, (7, 11)] = -1.0
+    q = torch.randn(rows, kv, G, hd, device="cuda")
+    q[..., 7], q[..., 11] = 1.0, 1.2  # 1.0 has nothing in its lower part, 1.2 something below zero
+    assert (q[..., 11].half().float() - q[..., 11] > 0).all()
+    k[-1, -1, :, 7] = -np.inf
+    none = n == 1  # the last row and head sees that block alone
+    cache, packed = _views(ops, table, np.arange(rows), np.full(rows, keys - 1), br, rows * n + 1, k, v)
+    out = torch.empty(rows, kv, G, hd, device="cuda")
+    sel = dev(np.tile(np.arange(n, dtype=np.int32), (rows, kv, 1)))
+    cache.attend(packed, q, sel, out)
+    torch.cuda.synchronize()
+    flat = lambda a: a[dev(table).long()].transpose(1, 2).reshape(rows, kv, keys, hd)  # noqa: E731
+    want, _ = _exact(q, flat(k), flat(v), hd ** -0.5)
+    if none:
+        assert want[-1, -1].isnan().all() and out[-1, -1].eq(0).all()
+        want[-1, -1] = 0.0
+    _, X = _exact(q, flat(k.nan_to_num(neginf=0.0)), flat(v), hd ** -0.5)
+    assert ((out.double() - want).abs() <= U * (11 * X + 20) * want).all()
+    k[int(table[0, 0]), 0, 0, 7] = np.inf
+    cache.attend(packed, q, sel, out)
+    torch.cuda.synchronize()
+    assert out[0, 0].isnan().all() and not out[1:].isnan().any()
