@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) paged_select_kernel(const b200
             tell(s_word + rank * kSelWarps + warp, __reduce_min_sync(0xffffffffu, kmin));
             tell(s_top + rank * kSelWarps + warp, __reduce_max_sync(0xffffffffu, kmax));
             everyone();
-            for (int i = 0; i < told; i++) {
+            for (int i = 0; i < ctas * kSelWarps; i++) {  // (one CTA that gathered tells itself alone)
                 kmin = min(kmin, s_word[i]);
                 kmax = max(kmax, s_top[i]);
             }
