@@ -413,8 +413,8 @@ int b200_paged_append(b200_ctx* ctx, const b200_paged_cache* cache, const b200_p
  * sel [n_rows][n_kv_heads][n_select], ascending, -1 behind the last: all of them when they are no more than n_select, else
  * the first n_first, the last n_recent (at least 1: the block being filled is not scored) and the best of those between by
  *     score = max over the group's query heads of sum_d q_d * (q_d > 0 ? largest_d : least_d),
- * the bound of q.k over the block's keys, compared in f64; ties go to the lower block. A NaN or infinite score counts as
- * the largest finite value, an unmapped block as the lowest. q [n_rows][ldq] f32, 16-byte aligned, ldq a multiple of 4; a
+ * the bound of q.k over the block's keys, compared in f64; ties go to the lower block. A NaN or a score of +infinity counts
+ * as the largest finite value, a score of -infinity and an unmapped block as the lowest. q [n_rows][ldq] f32, 16-byte aligned, ldq a multiple of 4; a
  * group has 1 to 8 query heads; n_select at most 2048, max_blocks at most 24576. */
 int b200_paged_select(b200_ctx* ctx, const b200_paged_cache* cache, const b200_paged_rows* rows, const float* q, int ldq, int n_heads,
                       int n_first, int n_recent, int n_select, int32_t* sel);

@@ -40,3 +40,26 @@ def test_select_with_hundreds_in_doubt(ops, rows, kv, G, hd, max_blocks, n_first
         cache.select(packed, torch.from_numpy(q).cuda(), sel, n_first=n_first, n_recent=n_recent)
         torch.cuda.synchronize()
         np.testing.assert_array_equal(sel.cpu().numpy(), _select_reference(q, bounds, table, slot, pos, br, kv, n_first, n_recent, n, before))
+
+
+@pytest.mark.parametrize("rows,kv,G,hd,max_blocks,n", [(1, 2, 4, 128, 90, 12), (3, 1, 8, 64, 700, 40), (40, 2, 2, 64, 30, 9)])
+def test_select_scores_of_minus_infinity_are_the_lowest(ops, rows, kv, G, hd, max_blocks, n):  # noqa: F811
+    """A block whose keys are all -inf in a dim where every query is above zero scores -inf: no more than an unmapped block, and less
+    than every other one. With too few others the lower of these is taken."""
+    rng = np.random.default_rng(max_blocks)
+    n_blocks, br = rows * max_blocks + 1, 16
+    bounds = np.sort(rng.normal(0, 1, (n_blocks, kv, 2, hd)), axis=2).astype(np.float16)
+    q = rng.normal(0, 1, (rows, kv, G, hd)).astype(np.float32)
+    q[..., 4] = np.abs(q[..., 4]) + 0.1
+    table = (1 + np.arange(rows * max_blocks, dtype=np.int32)).reshape(rows, max_blocks)
+    others = rng.permutation(max_blocks - 2)[:n // 2] + 1  # fewer than there is room for
+    low = np.setdiff1d(np.arange(1, max_blocks - 1), others)
+    bounds[table[:, low[::2]], :, :, 4] = -np.inf
+    table[:, low[1::2]] = 0
+    slot, pos = np.arange(rows, dtype=np.int32), np.full(rows, max_blocks * br - 1, np.int32)
+    cache, packed = _views(ops, table, slot, pos, br, n_blocks, key_bounds=torch.from_numpy(bounds).cuda())
+    sel = torch.zeros(rows, kv, n, dtype=torch.int32, device="cuda")
+    cache.select(packed, torch.from_numpy(q.reshape(rows, -1)).cuda(), sel)
+    torch.cuda.synchronize()
+    want = np.sort(np.concatenate(([0, max_blocks - 1], others, low[:n - 2 - len(others)])))
+    assert (sel.cpu().numpy() == want).all()
