@@ -29,6 +29,12 @@ def _refuse(text: str):
     raise ResidentError(abi.BAD_ARGUMENT, text)
 
 
+_vp, _i, _f = C.c_void_p, C.c_int, C.c_float
+# Foreign functions of this module's own: argument types set on the library's would hold for every other caller of it too.
+_CALLS = (("b200_paged_plan", C.CFUNCTYPE(_i, _vp, _vp, _vp, _vp, _vp)), ("b200_paged_append", C.CFUNCTYPE(_i, _vp, _vp, _vp, _vp, _i, _vp, _i)),
+          ("b200_paged_select", C.CFUNCTYPE(_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp)),
+          ("b200_paged_attend", C.CFUNCTYPE(_i, _vp, _vp, _vp, _vp, _i, _i, _f, _f, _vp, _i, _vp, _i)))
+
 _F32, _F16, _I32 = "torch.float32", "torch.float16", "torch.int32"
 _names: dict = {}  # dtype -> its text: formatting one costs more than a whole check
 
@@ -120,13 +126,7 @@ class PagedCache:
                                 _array("seq_blocks", seq_blocks, i32, (self.n_seqs,), dev), _array("free_blocks", free_blocks, i32, (n_blocks,), dev),
                                 _array("free_count", free_count, i32, (1,), dev), n_blocks, self.n_seqs, max_blocks, block_rows, kv, hd)
         self._c, self._drv = C.addressof(self.c), ops.drv
-        lib = ops.lib
-        vp, i, f = C.c_void_p, C.c_int, C.c_float
-        for fn, types in ((lib.b200_paged_plan, (vp, vp, vp, vp, vp)), (lib.b200_paged_append, (vp, vp, vp, vp, i, vp, i)),
-                          (lib.b200_paged_select, (vp, vp, vp, vp, i, i, i, i, i, vp)),
-                          (lib.b200_paged_attend, (vp, vp, vp, vp, i, i, f, f, vp, i, vp, i))):
-            fn.argtypes = types
-        self._plan, self._append, self._select, self._attend = lib.b200_paged_plan, lib.b200_paged_append, lib.b200_paged_select, lib.b200_paged_attend
+        self._plan, self._append, self._select, self._attend = (proto((name, ops.lib)) for name, proto in _CALLS)
 
     def _raise(self, st: int):
         raise ResidentError(st, self.ops.drv.last_error())
