@@ -36,6 +36,7 @@ _CALLS = (("b200_paged_plan", C.CFUNCTYPE(_i, _vp, _vp, _vp, _vp, _vp)), ("b200_
           ("b200_paged_attend", C.CFUNCTYPE(_i, _vp, _vp, _vp, _vp, _i, _i, _f, _f, _vp, _i, _vp, _i)))
 
 _F32, _F16, _I32 = "torch.float32", "torch.float16", "torch.int32"
+_I32_MAX = 2**31 - 1
 _names: dict = {}  # dtype -> its text: formatting one costs more than a whole check
 
 
@@ -61,9 +62,18 @@ def _array(name: str, a, dtype: str, shape, device: int) -> int:
     return a.data_ptr()
 
 
+def _int(name: str, n: int) -> int:
+    """n, for a 32-bit integer of the C call, which a foreign call would cut to its low bits."""
+    if n > _I32_MAX or n < -_I32_MAX:
+        _refuse(f"{name} is {n}, past 32 bits")
+    return n
+
+
 def _packed(name: str, a, n_rows: int, device: int):
     """Address, row stride and row width of a f32 [n_rows][...] device array whose rows are contiguous."""
     shape, stride = a.shape, a.stride()
+    if stride and stride[0] > _I32_MAX:
+        _refuse(f"the rows of {name} lie {stride[0]} values apart, past 32 bits")
     if len(shape) == 2 and stride[1] == 1 and shape[0] == n_rows and _names.get(a.dtype) == _F32 and a.get_device() == device:
         return a.data_ptr(), stride[0] if n_rows > 1 else shape[1], shape[1]
     if len(shape) < 2 or shape[0] != n_rows or not _is(a.dtype, _F32) or a.get_device() != device:
@@ -83,14 +93,15 @@ class PagedRows:
         device = row_slot.get_device()
         if device < 0:
             _refuse(f"row_slot is on {row_slot.device}")
-        n = row_slot.shape[0]
+        i32 = _I32
+        slots = _array("row_slot", row_slot, i32, (None,), device)
+        row0 = None if seq_row0 is None else _array("seq_row0", seq_row0, i32, (None,), device)
+        n = _int("the number of rows", row_slot.shape[0])
         self.n_rows, self.device = n, device
-        self.n_seqs = None if seq_row0 is None else seq_row0.shape[0] - 1
+        self.n_seqs = None if seq_row0 is None else _int("the number of sequences", seq_row0.shape[0] - 1)
         self._keep = (row_slot, row_pos, slot_map, seq_row0, status)
         self.row_slot, self.row_pos, self.slot_map, self.seq_row0, self.status = self._keep
-        i32 = _I32
-        self.c = abi.PagedRows(None if seq_row0 is None else _array("seq_row0", seq_row0, i32, (None,), device),
-                               _array("row_slot", row_slot, i32, (n,), device), _array("row_pos", row_pos, i32, (n,), device),
+        self.c = abi.PagedRows(row0, slots, _array("row_pos", row_pos, i32, (n,), device),
                                None if slot_map is None else _array("slot_map", slot_map, i32, (n,), device),
                                None if status is None else _array("status", status, i32, (4,), device), n, 0)
         self._c = C.addressof(self.c)
@@ -106,8 +117,10 @@ class PagedCache:
         dev, i32, f16 = self.device, _I32, _F16
         self._keep = (block_table, seq_blocks, free_blocks, free_count, k_pool, v_pool, key_bounds)
         table = _array("block_table", block_table, i32, (None, None), dev)
-        self.n_seqs, max_blocks = block_table.shape
-        n_blocks = free_blocks.shape[0]
+        stack = _array("free_blocks", free_blocks, i32, (None,), dev)
+        self.n_seqs, max_blocks = (_int("an extent of block_table", n) for n in block_table.shape)
+        n_blocks = _int("the number of blocks", free_blocks.shape[0])
+        _int("block_rows", block_rows)
         kv = hd = 0
         if k_pool is not None or v_pool is not None:
             if k_pool is None or v_pool is None:
@@ -119,11 +132,12 @@ class PagedCache:
             if len(key_bounds.shape) != 4:
                 _refuse(f"key_bounds has shape {tuple(key_bounds.shape)}, not [n_blocks][n_kv_heads][2][head_dim]")
             kv, hd = key_bounds.shape[1], key_bounds.shape[3]
+        _int("the number of kv heads", kv), _int("head_dim", hd)
         pool = lambda name, a: None if a is None else _array(name, a, f16, (n_blocks, kv, block_rows, hd), dev)  # noqa: E731
         self.block_rows, self.n_kv_heads, self.head_dim = block_rows, kv, hd
         self.c = abi.PagedCache(pool("k_pool", k_pool), pool("v_pool", v_pool),
                                 None if key_bounds is None else _array("key_bounds", key_bounds, f16, (n_blocks, kv, 2, hd), dev), table,
-                                _array("seq_blocks", seq_blocks, i32, (self.n_seqs,), dev), _array("free_blocks", free_blocks, i32, (n_blocks,), dev),
+                                _array("seq_blocks", seq_blocks, i32, (self.n_seqs,), dev), stack,
                                 _array("free_count", free_count, i32, (1,), dev), n_blocks, self.n_seqs, max_blocks, block_rows, kv, hd)
         self._c, self._drv = C.addressof(self.c), ops.drv
         self._plan, self._append, self._select, self._attend = (proto((name, ops.lib)) for name, proto in _CALLS)
@@ -163,8 +177,10 @@ class PagedCache:
     def select(self, rows: PagedRows, q, sel, n_first: int = 1, n_recent: int = 1):
         n, device = self._here(rows), self.device
         pq, ldq, width = _packed("q", q, n, device)
-        n_select = sel.shape[-1]
+        n_select = sel.shape[-1] if sel.shape else 0
         ps = _array("sel", sel, _I32, (n, self.n_kv_heads, n_select), device)
+        if n_select > _I32_MAX or not -_I32_MAX <= n_first <= _I32_MAX or not -_I32_MAX <= n_recent <= _I32_MAX:
+            _refuse(f"lists of {n_select} blocks with the first {n_first} and the last {n_recent}")
         st = self._select(self._drv.ctx.value, self._c, rows._c, pq, ldq, self._heads("q", width), n_first, n_recent, n_select, ps)
         if st:
             self._raise(st)
@@ -175,8 +191,10 @@ class PagedCache:
         po, ldo, wide = _packed("out", out, n, device)
         if wide != width:
             _refuse(f"out has shape {tuple(out.shape)}, q {tuple(q.shape)}")
-        n_select = sel.shape[-1]
+        n_select = sel.shape[-1] if sel.shape else 0
         ps = _array("sel", sel, _I32, (n, self.n_kv_heads, n_select), device)
+        if n_select > _I32_MAX:
+            _refuse(f"lists of {n_select} blocks")
         st = self._attend(self._drv.ctx.value, self._c, rows._c, pq, ldq, self._heads("q", width), scale, softcap, ps, n_select, po, ldo)
         if st:
             self._raise(st)
