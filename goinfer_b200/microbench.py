@@ -41,10 +41,18 @@ def paged(args):
         one = torch.ones_like(length)
         k, q = torch.randn(n, kv, hd, device="cuda"), torch.randn(n, args.heads, hd, device="cuda")
         sel, out = i32(n, kv, args.select), torch.empty_like(q)
-        scored = int((torch.where(blocks > args.select, blocks - 2, 0)).sum()) * kv
-        read = int(torch.minimum(torch.minimum(blocks, torch.tensor(args.select)) * br, length.cpu() + 1).sum()) * kv
-        for name, call, nbytes in (("plan", lambda: cache.plan(length, one, rows), 4 * 9 * n), ("append", lambda: cache.append(rows, k, k), 12 * k.numel()),
-                                   ("select", lambda: cache.select(rows, q, sel), 4 * hd * scored), ("attend", lambda: cache.attend(rows, q, sel, out), 4 * hd * read)):
+        v = torch.randn_like(k)
+        # what a call cannot do without. plan: lengths and blocks in, blocks and first rows out, three numbers a row; append: k and v in and
+        # stored, the slots, the bounds out, a block's older keys for them; select and attend: queries and lists, the bounds of the
+        # blocks between the first and the last, the keys and values of the listed rows (a row's last block is among them), the outputs
+        older = int((length % br).sum())
+        scored = int((torch.where(blocks.cuda() > args.select, blocks.cuda() - 2, 0)).sum()) * kv
+        read = int((blocks.clamp_max(args.select) * br - (blocks * br - length.cpu() - 1)).sum()) * kv
+        asked = 4 * (q.numel() + sel.numel())
+        for name, call, nbytes in (("plan", lambda: cache.plan(length, one, rows), 4 * 8 * n),
+                                   ("append", lambda: cache.append(rows, k, v), 12 * k.numel() + 4 * n + 4 * k.numel() + 2 * kv * hd * older),
+                                   ("select", lambda: cache.select(rows, q, sel), asked + 4 * hd * scored),
+                                   ("attend", lambda: cache.attend(rows, q, sel, out), asked + 4 * q.numel() + 4 * hd * read)):
             for _ in range(args.warmup):
                 call()
             a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
