@@ -20,18 +20,17 @@
 //
 // Weights. hi + lo is x to 2^-22 where the step of fp16's subnormals, 2^-24, is no more than 2^-21 of x: for x >= 2^-3. A weight is
 // taken in 2^-15ths, p = 2^15 exp(x - m) <= 32768, in the context and in the sum alike, so this holds for those down to 2^-18 of the
-// largest one that the warp has seen. Where a tile has smaller ones (a key 12.5 above the rest, say, whose own value may be
-// next to nothing), they are left out of the first product and multiplied by V again, 2^18 times as large, until none is left: every
-// weight keeps its 2^-22 down to the smallest numbers of fp32. The look costs 1 % at head_dim 128 and nothing at 64 (256 rows of 128
-// blocks 312.6 -> 313.5 us, 45 ragged rows 11.9 either way); where every tile has such weights, the second product takes 329 us in place of
-// 313, 14 in place of 12.
+// largest one that the warp has seen. Where a tile has a score 12.4 or more below the largest (a key far above the rest, say, whose
+// own value may be next to nothing), what the halves left of the weights below 2^-3 is multiplied by V once more, 2^36 times as large, until
+// none is below: every weight keeps its 2^-22 down to the smallest numbers of fp32. Measured against no care at all: the look costs up to
+// 1 % (256 rows of 128 blocks 312.5 -> 313.2 us, 45 ragged rows 12.0 -> 12.3); where every tile has such a score 317 and 14.1 us.
 #include "paged.cuh"
 
 namespace {
 
 constexpr int kAttWarps = 4, kAttThreads = 32 * kAttWarps, kAttStages = 2;
 constexpr int kAttMaxList = 2048;
-constexpr float kWeight = 0x1p15f, kSmall = 0x1p-3f, kStep = 0x1p18f;  // of the weights, see above
+constexpr float kWeight = 0x1p15f, kSmall = 0x1p-3f, kStep = 0x1p36f, kFar = -12.4f;  // of the weights, see above; 2^-18 = exp(-12.48)
 constexpr int kAttMaxCluster = 8;
 
 __device__ __forceinline__ void ldm4(unsigned addr, unsigned (&r)[4]) {
@@ -218,11 +217,12 @@ __global__ void __launch_bounds__(kAttThreads, HD == 64 ? 4 : 2) paged_attend_ke
         auto joined = [](float hi, float lo) { return fabsf(hi) == INFINITY ? hi : fmaf(lo, 0x1p-11f, hi); };
         float x[4] = {joined(s0h[0], s0l[0]), joined(s0h[1], s0l[1]), joined(s1h[0], s1l[0]), joined(s1h[1], s1l[1])};
         const int kk[4] = {key0 + 2 * tig, key0 + 2 * tig + 1, key0 + 8 + 2 * tig, key0 + 9 + 2 * tig};
-        float mx = -INFINITY;
+        float mx = -INFINITY, least = INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             x[i] *= scale;  // this lane's scores are all of head gid
             if (cap != 0.f) x[i] = cap * tanhf(x[i] * inv_cap);
+            least = fminf(least, x[i]);  // (of keys that the row does not see as well)
             if (kk[i] >= n_keys) x[i] = -INFINITY;
             mx = fmaxf(mx, x[i]);
         }
@@ -232,21 +232,19 @@ __global__ void __launch_bounds__(kAttThreads, HD == 64 ? 4 : 2) paged_attend_ke
         const float m_ref = m_new == -INFINITY ? 0.f : m_new;  // nothing seen yet: every weight is exp(-inf) = 0
         const float alpha = __expf(m_run - m_ref);
         float p[4], ps = 0.f;
-        bool small = false;  // a weight that two halves do not hold to 2^-22
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             p[i] = kWeight * __expf(x[i] - m_ref);
             ps += p[i];
-            small |= p[i] > 0.f && p[i] < kSmall;
         }
-        small = __any_sync(0xffffffffu, small);
         ps += __shfl_xor_sync(0xffffffffu, ps, 1);
         ps += __shfl_xor_sync(0xffffffffu, ps, 2);
         l_run = l_run * alpha + ps;
         m_run = m_new;
         unsigned ph0, pl0, ph1, pl1;
-        split2(p[0] < kSmall ? 0.f : p[0], p[1] < kSmall ? 0.f : p[1], ph0, pl0);
-        split2(p[2] < kSmall ? 0.f : p[2], p[3] < kSmall ? 0.f : p[3], ph1, pl1);
+        split2(p[0], p[1], ph0, pl0);
+        split2(p[2], p[3], ph1, pl1);
+        const bool far = __any_sync(0xffffffffu, least - m_ref < kFar);  // a weight below kSmall, perhaps
         const float a0 = __shfl_sync(0xffffffffu, alpha, (2 * tig) * 4), a1 = __shfl_sync(0xffffffffu, alpha, (2 * tig + 1) * 4);
 #pragma unroll
         for (int mt = 0; mt < KS; mt++) {
@@ -260,30 +258,32 @@ __global__ void __launch_bounds__(kAttThreads, HD == 64 ? 4 : 2) paged_attend_ke
             o[mt][2] = fmaf(o[mt][2], a0, d[2]);
             o[mt][3] = fmaf(o[mt][3], a1, d[3]);
         }
-        for (float down = 1.f; small;) {  // at most eight times: 2^-149 * 2^15 is then above 2^-3
-            down *= 1.f / kStep;
-            bool here = false;
-            small = false;
+        if (far) {
+            bool more = true;  // at most four times: 2^-149 * 2^15 * 2^144 is above kSmall
+            for (float down = 1.f / kStep; more; down *= 1.f / kStep) {
+                auto left = [](float x, float y, unsigned hi, unsigned lo, float& a, float& b) {
+                    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi)), l = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+                    a = fabsf(x) < kSmall ? ((x - h.x) - l.x) * kStep : 0.f;
+                    b = fabsf(y) < kSmall ? ((y - h.y) - l.y) * kStep : 0.f;
+                };
+                left(p[0], p[1], ph0, pl0, p[0], p[1]);
+                left(p[2], p[3], ph1, pl1, p[2], p[3]);
+                more = false;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                p[i] = p[i] < kSmall ? p[i] * kStep : 0.f;  // (those of the step before are done, a NaN was in the first)
-                here |= p[i] >= kSmall;
-                small |= p[i] > 0.f && p[i] < kSmall;
-            }
-            here = __any_sync(0xffffffffu, here);
-            small = __any_sync(0xffffffffu, small);
-            if (!here) continue;
-            split2(p[0] < kSmall ? 0.f : p[0], p[1] < kSmall ? 0.f : p[1], ph0, pl0);
-            split2(p[2] < kSmall ? 0.f : p[2], p[3] < kSmall ? 0.f : p[3], ph1, pl1);
+                for (int i = 0; i < 4; i++) more |= p[i] != 0.f && fabsf(p[i]) < kSmall;
+                more = __any_sync(0xffffffffu, more);
+                split2(p[0], p[1], ph0, pl0);
+                split2(p[2], p[3], ph1, pl1);
 #pragma unroll
-            for (int mt = 0; mt < KS; mt++) {
-                unsigned v[4];
-                ldm4_t(vb + (unsigned)(lrow * ROWB + (((2 * mt + lsel) ^ (lrow & 7)) << 4)), v);
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816(d, v[0], v[1], v[2], v[3], pl0, pl1);
-                mma16816(d, v[0], v[1], v[2], v[3], ph0, ph1);
+                for (int mt = 0; mt < KS; mt++) {
+                    unsigned v[4];
+                    ldm4_t(vb + (unsigned)(lrow * ROWB + (((2 * mt + lsel) ^ (lrow & 7)) << 4)), v);
+                    float d[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma16816(d, v[0], v[1], v[2], v[3], pl0, pl1);
+                    mma16816(d, v[0], v[1], v[2], v[3], ph0, ph1);
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[mt][i] = fmaf(d[i], down, o[mt][i]);
+                    for (int i = 0; i < 4; i++) o[mt][i] = fmaf(d[i], down, o[mt][i]);
+                }
             }
         }
         __syncwarp();
