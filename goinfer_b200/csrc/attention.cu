@@ -179,6 +179,9 @@ __global__ void __launch_bounds__(128) attn_split_kernel(const float* __restrict
 // product keeps fp32-level accuracy over the fp16 keys); the context is accumulated transposed, O^T[dim][head] = V^T P^T,
 // so that the score fragment of a lane is already the B fragment of the second product and the 8-column operand holds
 // the (up to 8) heads of the group. Online softmax in fp32 registers; P is also split hi + lo. G <= 8.
+// The halves share fp16's smallest step, 2^-24, so a weight is taken in 2^-15ths (at most 32768), in the context and in the sum alike:
+// it keeps 2^-22 of itself down to 2^-18 of the largest one of the warp's keys so far, and 2^-40 of that one below (unscaled, a key
+// that scored 18 above the others, with a value of zero, took the rest of its warp's part of the split with it).
 __device__ __forceinline__ void ldsm_x4(unsigned addr, unsigned& r0, unsigned& r1, unsigned& r2, unsigned& r3) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
 }
@@ -204,6 +207,7 @@ __device__ __forceinline__ void split_hi_lo(float x, float y, unsigned& hi, unsi
 }
 
 constexpr int kMmaStages = 3;
+constexpr float kWeight = 0x1p15f;
 
 template <int HD, int G>
 __global__ void __launch_bounds__(128) attn_mma_kernel(const float* __restrict__ q, int ldq, int nH, int nKV, float scale, float cap,
@@ -301,7 +305,7 @@ __global__ void __launch_bounds__(128) attn_mma_kernel(const float* __restrict__
         float pv[4], ps = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            pv[i] = __expf(sv[i] - m_new);   // exp(-inf) = 0 for masked keys
+            pv[i] = kWeight * __expf(sv[i] - m_new);   // exp(-inf) = 0 for masked keys
             ps += pv[i];
         }
         ps += __shfl_xor_sync(0xffffffffu, ps, 1);
