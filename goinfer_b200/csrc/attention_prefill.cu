@@ -8,7 +8,9 @@
 // by the warps, 16-byte chunks XOR-swizzled by key row) are fetched once per group. Per warp and tile:
 //   S[16 rows][32 keys] = Q K^T   mma.sync m16n8k16, Q held in registers as f16 hi + lo parts (fp32-level accuracy)
 //   online softmax in fp32 registers (rows gid and gid+8 of the lane's quad)
-//   O[16][HD] += P V              P = the S accumulators re-used as the A fragment, split hi + lo as well
+//   O[16][HD] += P V              P = the S accumulators re-used as the A fragment, split hi + lo as well, in 2^-15ths: the halves
+//                                 share fp16's smallest step, so a weight keeps 2^-22 of itself down to 2^-18 of the row's largest
+//                                 and 2^-40 of that one below
 // The walk is flash-attention style, one pass over the keys, nothing written but the final rows. The arithmetic is the
 // decode kernel's (same splits, same fp32 softmax); only the grouping of rows differs.
 #include <cstdlib>
@@ -16,6 +18,8 @@
 #include "common.cuh"
 
 namespace {
+
+constexpr float kPfWeight = 0x1p15f;
 
 __device__ __forceinline__ float pf_score(float dot, float scale, float cap) {
     float s = dot * scale;
@@ -163,8 +167,8 @@ __global__ void __launch_bounds__(32 * G) attn_prefill_kernel(const float* __res
             ps_a += p0 + p1;
             ps_b += p2 + p3;
             // key group j is columns (j&1)*8.. of step j>>1: a0/a1 for the low half, a2/a3 for the high half
-            pf_split(p0, p1, ph[j >> 1][(j & 1) * 2], pl[j >> 1][(j & 1) * 2]);
-            pf_split(p2, p3, ph[j >> 1][(j & 1) * 2 + 1], pl[j >> 1][(j & 1) * 2 + 1]);
+            pf_split(kPfWeight * p0, kPfWeight * p1, ph[j >> 1][(j & 1) * 2], pl[j >> 1][(j & 1) * 2]);
+            pf_split(kPfWeight * p2, kPfWeight * p3, ph[j >> 1][(j & 1) * 2 + 1], pl[j >> 1][(j & 1) * 2 + 1]);
         }
         ps_a += __shfl_xor_sync(0xffffffffu, ps_a, 1);
         ps_a += __shfl_xor_sync(0xffffffffu, ps_a, 2);
@@ -193,7 +197,7 @@ __global__ void __launch_bounds__(32 * G) attn_prefill_kernel(const float* __res
         }
     }
     asm volatile("cp.async.wait_group 0;\n" ::);
-    const float inv_a = 1.f / l_a, inv_b = 1.f / l_b;
+    const float inv_a = 1.f / (kPfWeight * l_a), inv_b = 1.f / (kPfWeight * l_b);
     if (r0 + gid < nrows) {
         float* op = out + (size_t)(r0 + gid) * ldo + (size_t)head * HD;
 #pragma unroll
