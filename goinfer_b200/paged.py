@@ -72,7 +72,7 @@ def _int(name: str, n: int) -> int:
 def _packed(name: str, a, n_rows: int, device: int):
     """Address, row stride and row width of a f32 [n_rows][...] device array whose rows are contiguous."""
     shape, stride = a.shape, a.stride()
-    if stride and stride[0] > _I32_MAX:
+    if n_rows > 1 and stride and stride[0] > _I32_MAX:
         _refuse(f"the rows of {name} lie {stride[0]} values apart, past 32 bits")
     if len(shape) == 2 and stride[1] == 1 and shape[0] == n_rows and _names.get(a.dtype) == _F32 and a.get_device() == device:
         return a.data_ptr(), stride[0] if n_rows > 1 else shape[1], shape[1]

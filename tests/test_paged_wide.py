@@ -66,3 +66,13 @@ def test_arrays_without_extents(lib, host):  # noqa: F811
     _refused(c.select, r, q, none)
     _refused(c.attend, r, q, none, Array((3, 512)))
     _refused(c.attend, r, q, sel, Array(()))
+
+
+def test_the_stride_of_a_single_row_does_not_count(lib, host):  # noqa: F811
+    c, r = _view(lib, host), _packed(row_slot=i32(1), row_pos=i32(1), slot_map=i32(1))
+    far = Array((1, 128), stride=(W + 128, 1))
+    for call in (lambda: c.append(r, far, far), lambda: c.select(r, Array((1, 8, 64), stride=(W, 64, 1)), i32(1, 2, 4)),
+                 lambda: c.attend(r, Array((1, 512), stride=(W, 1)), i32(1, 2, 4), Array((1, 512)))):
+        with pytest.raises(ResidentError) as e:
+            call()
+        assert e.value.status == abi.CUDA_ERROR, e.value  # accepted, and the context has no device
