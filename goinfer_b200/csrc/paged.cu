@@ -362,10 +362,13 @@ extern "C" int b200_paged_plan(b200_ctx* ctx, const b200_paged_cache* c, const b
     const size_t scan = sizeof(int) * ((size_t)c->n_seqs + 1);
     CUDA_TRY(ctx, limit.raise(paged_plan_kernel, ctx->device, 3 * sizeof(int) * (kPlanMaxSeqs + 1)));
     const bool apart = r->n_rows > 2 * kPlanThreads;
-    // sequences and blocks enough for four a thread: a cluster (2000 sequences with 64000 rows, both calls of a round: 17.3 against
-    // 21.8 us with one CTA)
+    // Sequences and blocks enough for four a thread: a cluster. Two calls with a cluster and with one CTA, in us, sequences x rows: 2000 x
+    // 32 16.5 and 21.4, 1000 x 60 14.0 and 17.9, 5000 x 8 22.8 and 27.4, 5000 x 1 21.1 and 21.9, 4000 x 1 19.4 and 18.9; below the
+    // border 2000 x 1 13.9 and 13.5, 64 x 1 8.9 and 7.0, 1000 x 30 14.2 either way, but 256 x 200 12.0 and 14.6.
     const int ctas = c->n_seqs + r->n_rows / c->block_rows > 4 * kPlanThreads ? 8 : 1;
-    // a decode step's lengths do with eight warps, whose barriers are the cheaper (64 sequences: 6.1 against 6.7 us for two calls)
+    // A decode step's lengths do with eight warps, whose barriers are the cheaper. Two calls with 8 and with 32 warps: 1 sequence of 1 row 5.6
+    // and 6.4 us, 64 x 1 6.1 and 7.0, 256 x 1 7.0 and 7.6, 64 x 8 7.1 and 7.2; behind the border 256 x 2 8.0 and 7.7, 300 x 1 9.0 and
+    // 7.9, 1000 x 1 13.1 and 9.6.
     const int threads = c->n_seqs <= 256 && r->n_rows <= 512 ? 256 : kPlanThreads;
     launch_cluster(paged_plan_kernel, ctas, dim3(ctas), dim3(threads), 3 * scan, ctx->stream, a, apart ? 0 : 1);
     if (apart) {
@@ -392,10 +395,15 @@ extern "C" int b200_paged_append(b200_ctx* ctx, const b200_paged_cache* c, const
     DeviceScope dev;
     CUDA_TRY(ctx, dev.enter(ctx->device));
     // Few rows are decode steps: a CTA looks at one, and while there is an SM for each, with tall blocks sixteen warps share the
-    // older rows to be read. Many rows are prompts, whose runs fill blocks: a CTA that finds no run among its rows costs about
-    // as much as 4 ns of the GPU, so it looks at more, as long as four CTAs an SM are left (32768 rows of 8 heads of 128 in
-    // blocks of 64: 139, 82, 74, 68 us with 1, 4, 8, 32 rows a CTA; 2115 rows in seven chunks with blocks of 32: 8.1, 5.3, 5.5,
-    // 7.2 us; 5529 rows of one head of 64 in 291 chunks: 6.9 us with 16, 8.4 with 32).
+    // older rows to be read. With sixteen and with eight warps, 64 decode rows of 8 heads of 128 in blocks of 16, 32, 64, 256: 3.5 and 3.4,
+    // 3.8 and 4.1, 4.4 and 5.1, 8.7 and 12.6 us; of 4 heads of 64 in blocks of 32, 64, 128, 256: 3.4 and 3.3, 3.6 and 3.5, 3.9 and
+    // 4.1, 4.6 and 5.2; 200 rows of 8 heads of 128 in blocks of 64, 256: 7.3 and 5.8, 22.5 and 27.7. (What decides is how many CTAs hold a
+    // run, which the rows alone do not say: seven chunks of 301 rows of 8 heads of 128 would take 12.9 us with sixteen, 17.4 with eight, in
+    // blocks of 64; of 4 heads of 64 in blocks of 32 5.9 and 4.9.)
+    // Many rows are prompts, whose runs fill blocks: a CTA that finds no run among its rows costs about as much as 4 ns of the GPU, so it
+    // looks at more, as long as four CTAs an SM are left (32768 rows of 8 heads of 128 in blocks of 64: 139, 82, 74, 68 us with 1, 4, 8, 32
+    // rows a CTA; 2115 rows in seven chunks with blocks of 32: 8.1, 5.3, 5.5, 7.2 us; 5529 rows of one head of 64 in 291 chunks: 6.9 us
+    // with 16, 8.4 with 32).
     int rows = 1;
     while (rows < 32 && r->n_rows > 4 * ctx->sm_count * rows) rows *= 2;
     const int warps = r->n_rows <= ctx->sm_count && c->block_rows >= 32 ? kAppendMaxWarps : 8;

@@ -71,7 +71,8 @@ struct AttendShape {
 
 // Two CTAs an SM at least: with all the registers that leaves it the compiler keeps more of a tile's steps in flight than it would
 // by itself (4 x 131k keys 45.6 against 49.7 us; 256 rows 312 against 310). Four at head_dim 64: 128 registers, where the compiler takes
-// 137 by itself (128 rows of 64 blocks 25.1 against 27.7 us).
+// 135 by itself and three fit (32/4 heads, 128 rows of 64 blocks 25.2 against 33.1 us, 256 rows 47.1 against 54.3; 200 rows, which then
+// happen to fill the last wave, 44.2 against 38.7).
 template <int HD>
 __global__ void __launch_bounds__(kAttThreads, HD == 64 ? 4 : 2) paged_attend_kernel(const b200_paged_cache c, const int32_t* row_slot,
                                                                    const int32_t* row_pos, const float* q, size_t ldq, int G,

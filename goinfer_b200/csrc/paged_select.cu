@@ -11,9 +11,11 @@
 // blocks each, where the bytes take 42). So the scores are first taken on the matrix unit, with a bound of their error:
 //     s~ = sum_{q > 0} q_d hi_d + sum_{q <= 0} q_d lo_d     as mma.sync m16n8k16: 16 blocks x 8 heads x 16 dims,
 // q scaled by a power of two (largest |q| in [1, 2)) and split into fp16 parts hi + 2^-11 lo, products exact, fp32 sums. The
-// split leaves at most 2^-22 |q_d| or 2^-36; a step that adds 16 products to the sum is off by at most 17 * 2^-23 of the terms'
-// absolute sum S, the eight steps of either sum by 2^-15.9 S. E = 2^-14 S + 2^-12 covers it (128 dims of the largest fp16 bound
-// times 2^-36 are 2^-13), with S = sum |q_d| max(|lo_d|, |hi_d|), which is no less than the terms' sum, from the same unit. The true m-th
+// split leaves at most 2^-22 |q_d| or 2^-36. No document says how the unit rounds; assumed is that a step which adds 16 products to the
+// sum is off by at most 17 * 2^-23 of the terms' absolute sum S, one unit in the last place for each term cut off (observed: 2.3 * 2^-23 at
+// most, over 12 million steps with terms alike, of one sign, and 2^56 apart), and the eight steps of either sum by 2^-15.9 S.
+// E = 2^-14 S + 2^-12 covers it (128 dims of the largest fp16 bound times 2^-36 are 2^-13), with S = sum |q_d| max(|lo_d|, |hi_d|), which is
+// no less than the terms' sum, from the same unit. The true m-th
 // score lies within E of the m-th s~, so a block whose s~ is more than 2E above (below) that is in (out) for certain; only
 // the blocks between (a handful) are scored in f64. An infinity or a NaN anywhere makes E infinite, and every block is
 // scored in f64.

@@ -424,8 +424,11 @@ int b200_paged_select(b200_ctx* ctx, const b200_paged_cache* cache, const b200_p
  * twice counts twice). Scores are scale * q.k (scale 0: 1/sqrt(head_dim)), softcap > 0 (at least 1e-30) caps them
  * (decoder/attention.go:287-295);
  * a row that sees no key gets zeros. q [n_rows][ldq] and out [n_rows][ldo] f32, 16-byte aligned, strides a multiple of 4,
- * out apart from the inputs. fp32 accuracy over the fp16 cache. The same call on the same GPU gives the same bits; a list is
- * split by the number of rows and by what the GPU holds at once, so in a batch of another size a row's last bits may differ. */
+ * out apart from the inputs. fp32 accuracy over the fp16 cache: a weight keeps 2^-22 of itself however far below the largest it
+ * lies, a query 2^-22 of itself or 2^-36 of its head's largest. A key that makes a score -infinity has weight 0 (against a query
+ * of at least 2^-24 of its head's largest; NaN against a smaller one); a score that is +infinity or NaN makes the head's output
+ * NaN, a value of +-infinity that dim of it infinite or NaN. The same call on the same GPU gives the same bits; a list is split
+ * by the number of rows and by what the GPU holds at once, so in a batch of another size a row's last bits may differ. */
 int b200_paged_attend(b200_ctx* ctx, const b200_paged_cache* cache, const b200_paged_rows* rows, const float* q, int ldq, int n_heads,
                       float scale, float softcap, const int32_t* sel, int n_select, float* out, int ldo);
 
